@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_float, c_int, c_int32, c_size_t, c_void_p
+from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 from . import build as _build
 
@@ -21,12 +21,18 @@ EXPORTED = (
     "b200l_block_forward", "b200l_row_layernorm", "b200l_cast_f16",
     "b200l_kernel_workspace_bytes", "b200l_debug_arm", "b200l_noalloc_read_status",
     "b200l_convert",
+    "b200l_kv_plan", "b200l_kv_append", "b200l_kv_read",
+    "b200l_kv_attention_workspace_bytes", "b200l_kv_attention",
 )
 
 # Element types of b200l_convert.
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
-ABI_VERSION = 4
+ABI_VERSION = 5
+
+# Codes of the paged key/value cache.
+KV_INT8, KV_E4M3 = 0, 1
+KV_MAX_REQUESTS = 16384
 
 # Fault-injection sites of b200l_debug_arm (test hook for the bounded waits).
 DEBUG_SITE_NONE = 0
@@ -69,6 +75,47 @@ class BlockDesc(ctypes.Structure):
     ]
 
 
+class KVCacheDesc(ctypes.Structure):
+    """Mirror of ``b200l_kv_cache``."""
+
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("num_pages", c_int64), ("num_heads", c_int32), ("page_size", c_int32),
+        ("head_dim", c_int32), ("kind", c_int32),
+    ]
+
+
+class KVPlanDesc(ctypes.Structure):
+    """Mirror of ``b200l_kv_plan_desc``."""
+
+    _fields_ = [
+        ("old_lens", c_void_p), ("new_lens", c_void_p), ("block_table", c_void_p), ("table_stride", c_int64),
+        ("free_pages", c_void_p), ("free_count", c_void_p), ("cu_new", c_void_p), ("cu_pages", c_void_p),
+        ("positions", c_void_p), ("slots", c_void_p), ("info", c_void_p),
+        ("requests", c_int32), ("table_width", c_int32), ("page_size", c_int32), ("capacity", c_int32),
+        ("max_tokens", c_int32),
+    ]
+
+
+class KVRows(ctypes.Structure):
+    """Mirror of ``b200l_kv_rows``."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3),
+                ("dtype", c_int32)]
+
+
+class KVAttnDesc(ctypes.Structure):
+    """Mirror of ``b200l_kv_attn_desc``."""
+
+    _fields_ = [
+        ("q", c_void_p), ("out", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64),
+        ("block_table", c_void_p), ("table_stride", c_int64),
+        ("seq_lens", c_void_p), ("cu_new", c_void_p), ("cu_pages", c_void_p),
+        ("requests", c_int32), ("table_width", c_int32), ("tokens", c_int32), ("num_heads", c_int32),
+        ("max_new", c_int32), ("causal", c_int32), ("dtype", c_int32), ("scale", c_float),
+    ]
+
+
 class B200LError(RuntimeError):
     """A C-ABI call returned a negative status."""
 
@@ -103,6 +150,11 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200l_debug_arm": (c_int, [P, c_int32, ctypes.c_uint64, P]),
         "b200l_noalloc_read_status": (c_int, [P]),
         "b200l_convert": (c_int, [P, c_int32, P, c_int32, ctypes.c_int64, P]),
+        "b200l_kv_plan": (c_int, [P, P]),
+        "b200l_kv_append": (c_int, [P, P, P, c_int64, P]),
+        "b200l_kv_read": (c_int, [P, P, c_int64, P, P, c_int32, P]),
+        "b200l_kv_attention_workspace_bytes": (c_size_t, [P, P]),
+        "b200l_kv_attention": (c_int, [P, P, P, c_size_t, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -924,3 +924,6 @@ extern "C" int b200l_noalloc_read_status(void* stream) {
   if (rc) return rc;
   return b200l_read_status(ws, stream);
 }
+
+// ===================================================================== paged 8-bit key/value cache
+#include "kv_capi.cuh"

@@ -1,0 +1,330 @@
+"""A paged key/value cache in 8 bits, and attention over it.
+
+A causal model that has attended to a sequence can go on from it one token (or
+one chunk) at a time if it keeps the sequence's keys and values. Here they are
+kept as int8 or e4m3 codes with one fp32 scale per page of tokens and head, in
+pages that a block table hands to requests. A step is
+
+    plan = kv_plan(old_lens, new_lens, block_table, free_pages, free_count, page_size=..., max_tokens=...)
+    kv_append(k, v, plan.slots, cache)                                            # per layer
+    ctx = kv_attention(q, cache, block_table, new_lens, plan, max_new=...)        # per layer
+
+with lengths, tables and slots on the GPU throughout: nothing here waits for
+the GPU, and every call can be captured in a CUDA graph. ``KVPool`` keeps the
+lengths, the table and the free pages between steps. All calls run on the
+current stream of their tensors' device through the sm_100a library
+(``include/cobra_b200.h``); there is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+
+PAGE_SIZES = (16, 32, 64, 128)
+_KINDS = {torch.int8: _lib.KV_INT8, torch.float8_e4m3fn: _lib.KV_E4M3}
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+class KVCache(NamedTuple):
+    """One layer's cache: codes ``[num_pages, heads, page_size, dhp]`` and fp32
+    scales ``[num_pages, heads]`` (dhp: ``padded_head_dim``)."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+class KVPlan(NamedTuple):
+    """What a step's lengths come to (``kv_plan``), on the GPU."""
+
+    cu_new: torch.Tensor      # int32 [requests + 1]: new tokens before each request
+    cu_pages: torch.Tensor    # int32 [requests + 1]: pages of requests with new tokens before each request
+    positions: torch.Tensor   # int32 [max_tokens]: each new token's position, -1 past the last
+    slots: torch.Tensor       # int64 [max_tokens]: page * page_size + place, -1 for none
+    info: torch.Tensor        # int32 [2]: free pages left, pages that were missing
+
+
+def padded_head_dim(head_dim: int) -> int:
+    """Columns of a cached row: head_dim rounded up to 32, 64, 128 or 256."""
+    if not 1 <= head_dim <= 256:
+        raise ValueError(f"head_dim must be in [1, 256], got {head_dim}")
+    return 32 if head_dim <= 32 else 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256
+
+
+def new_kv_cache(num_pages: int, num_heads: int, head_dim: int, *, page_size: int = 64,
+                 dtype: torch.dtype = torch.int8, device="cuda") -> KVCache:
+    """An empty cache of one layer (codes and scales zero)."""
+    if num_pages <= 0 or num_heads <= 0:
+        raise ValueError(f"num_pages and num_heads must be positive, got {num_pages}, {num_heads}")
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if dtype not in _KINDS:
+        raise TypeError(f"a cache holds torch.int8 or torch.float8_e4m3fn, got {dtype}")
+    shape = (num_pages, num_heads, page_size, padded_head_dim(head_dim))
+    k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2))
+    ks, vs = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
+    return KVCache(k, v, ks, vs)
+
+
+# ---------------------------------------------------------------- checks
+def _on(device: torch.device, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _ints(dtype: torch.dtype, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
+
+def _table_stride(table: torch.Tensor, requests: int) -> int:
+    if table.dtype != torch.int32:
+        raise TypeError(f"block_table must be torch.int32, got {table.dtype}")
+    if table.dim() != 2 or table.shape[0] != requests or table.shape[1] == 0:
+        raise ValueError(f"block_table must be [{requests}, width], got {tuple(table.shape)}")
+    width = table.shape[1]
+    if (width > 1 and table.stride(1) != 1) or (requests > 1 and table.stride(0) < width):
+        raise ValueError("block_table's rows must be contiguous and apart")
+    return table.stride(0) if requests > 1 else width
+
+
+def _cuda(t: torch.Tensor, name: str) -> torch.device:
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}: the cache runs only on CUDA (sm_100a) devices; there is no CPU path")
+    return t.device
+
+
+def _cache_desc(cache: KVCache, head_dim: int, device: torch.device) -> _lib.KVCacheDesc:
+    k, v, ks, vs = cache
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2]:
+        raise ValueError(f"cache shapes do not fit: codes {tuple(shape)}, {tuple(v.shape)}, "
+                         f"scales {tuple(ks.shape)}, {tuple(vs.shape)}")
+    kind = _KINDS.get(k.dtype)
+    if kind is None or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise TypeError(f"cache codes must be int8 or float8_e4m3fn and scales float32, got {k.dtype}, {v.dtype}, "
+                        f"{ks.dtype}, {vs.dtype}")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("cache tensors must be contiguous")
+    if k.device != device or v.device != device or ks.device != device or vs.device != device:
+        raise ValueError(f"cache tensors must be on {device}")
+    if shape[3] != padded_head_dim(head_dim):
+        raise ValueError(f"cache rows have {shape[3]} columns, head_dim {head_dim} needs {padded_head_dim(head_dim)}")
+    return _lib.KVCacheDesc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), shape[0], shape[1], shape[2],
+                            head_dim, kind)
+
+
+# ---------------------------------------------------------------- workspaces
+class _Workspace:
+    """A workspace of each (device, stream): calls on one stream run one after
+    another, so they can share it. A buffer that was outgrown is kept (a captured
+    graph may still use it); each is at least twice the one before."""
+
+    def __init__(self) -> None:
+        self._held: Dict[Tuple[int, int], list] = {}
+
+    def get(self, device: torch.device, stream: int, need: int) -> Tuple[int, int]:
+        key = (device.index, stream)
+        held = self._held.get(key)
+        if held is None:
+            held = self._held[key] = []
+        if not held or held[-1][2] < need:
+            size = max(need, 2 * held[-1][2] if held else 0)
+            buf = torch.empty(size + 1024, dtype=torch.uint8, device=device)
+            ptr = (buf.data_ptr() + 1023) // 1024 * 1024
+            _lib.check(_lib.lib().b200l_clear_status(ptr, stream))
+            held.append((buf, ptr, size))
+        return held[-1][1], held[-1][2]
+
+    def check(self) -> None:
+        for (index, stream), held in self._held.items():
+            with torch.cuda.device(index):
+                for _, ptr, _ in held:
+                    _lib.check(_lib.lib().b200l_read_status(ptr, stream))
+
+
+_workspace = _Workspace()
+
+
+def kv_check_status() -> None:
+    """Synchronise and raise if an attention kernel recorded a device-side
+    failure (a bounded wait that ran out) in a workspace of this module."""
+    _workspace.check()
+
+
+class _Current:
+    """The device as the current one, and its current stream's handle."""
+
+    __slots__ = ("device", "other")
+
+    def __init__(self, device: torch.device) -> None:
+        self.device = device
+        self.other = None
+
+    def __enter__(self) -> int:
+        if torch.cuda.current_device() != self.device.index:
+            self.other = torch.cuda.device(self.device)
+            self.other.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.other is not None:
+            self.other.__exit__(*exc)
+
+
+# ---------------------------------------------------------------- operators
+def kv_plan(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+            free_count: torch.Tensor, *, page_size: int, max_tokens: int) -> KVPlan:
+    """Block table and slots for a step that takes each request from
+    ``old_lens`` to ``new_lens`` cached tokens (int32 ``[requests]``; less than
+    before: pages are given back, 0: finished).
+
+    ``block_table`` (int32 ``[requests, width]``, rows may be strided) and the
+    stack ``free_pages`` (int32 ``[num_pages]``, ``free_count`` int32 ``[1]`` of
+    them free) are updated in place; entries that the call reads it does not
+    write, so a repeated call gives the same answer. The step is adopted by going
+    on from ``new_lens`` and ``info[0]``. Where ``info[1]`` pages were missing,
+    their table entries and slots are -1: plan again with other ``new_lens``.
+    ``max_tokens`` bounds the new tokens; entries past them are -1.
+    """
+    dev = _cuda(old_lens, "old_lens")
+    _on(dev, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_count=free_count)
+    _ints(torch.int32, old_lens=old_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count)
+    if old_lens.dim() != 1 or new_lens.shape != old_lens.shape or old_lens.numel() == 0:
+        raise ValueError(f"old_lens and new_lens must be [requests], got {tuple(old_lens.shape)}, {tuple(new_lens.shape)}")
+    R = old_lens.numel()
+    table_stride = _table_stride(block_table, R)
+    if free_pages.dim() != 1 or free_count.numel() != 1:
+        raise ValueError("free_pages must be one-dimensional and free_count a single number")
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if max_tokens < 0:
+        raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
+    with _Current(dev) as stream:
+        # One allocation: slots (8 bytes each) first, then the int32 outputs.
+        ints = 2 * max_tokens + max_tokens + 2 * (R + 1) + 2
+        buf = torch.empty(ints, dtype=torch.int32, device=dev)
+        slots = buf[:2 * max_tokens].view(torch.int64)
+        positions, cu_new, cu_pages, info = buf[2 * max_tokens:].split((max_tokens, R + 1, R + 1, 2))
+        desc = _lib.KVPlanDesc(
+            old_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+            table_stride,
+            free_pages.data_ptr(), free_count.data_ptr(), cu_new.data_ptr(), cu_pages.data_ptr(), positions.data_ptr(),
+            slots.data_ptr(), info.data_ptr(), R, block_table.shape[1], page_size, free_pages.numel(), max_tokens)
+        _lib.check(_lib.lib().b200l_kv_plan(ctypes.byref(desc), stream))
+    return KVPlan(cu_new, cu_pages, positions, slots, info)
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: KVCache) -> None:
+    """Quantises new keys and values ``[tokens, heads, head_dim]`` (fp32, fp16 or
+    bf16, any strides) into ``slots`` (int64 ``[tokens]``, < 0: not stored).
+
+    The tokens of a page share one scale per head: a page written from its first
+    place on gets the scale that its tokens need; later tokens grow it where they
+    need more, and the codes before them are moved to the new scale. The slots of
+    one page have to follow one another in ``slots``, as ``kv_plan`` makes them.
+    Values that are not finite make their page's scale not-a-number.
+    """
+    dev = _cuda(k, "k")
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError(f"k and v must be [tokens, heads, head_dim], got {tuple(k.shape)}, {tuple(v.shape)}")
+    dtype = _DTYPES.get(k.dtype)
+    if dtype is None or v.dtype != k.dtype:
+        raise TypeError(f"k and v must both be fp32, fp16 or bf16, got {k.dtype}, {v.dtype}")
+    T, H, dh = k.shape
+    _on(dev, v=v, slots=slots)
+    _ints(torch.int64, slots=slots)
+    if slots.dim() != 1 or slots.numel() < T:
+        raise ValueError(f"slots must be [at least {T}], got {tuple(slots.shape)}")
+    if cache.k.dim() == 4 and cache.k.shape[1] != H:
+        raise ValueError(f"k has {H} heads, the cache {cache.k.shape[1]}")
+    with _Current(dev) as stream:
+        c = _cache_desc(cache, dh, dev)
+        rows = _lib.KVRows(k.data_ptr(), v.data_ptr(), k.stride(), v.stride(), dtype)
+        _lib.check(_lib.lib().b200l_kv_append(ctypes.byref(c), ctypes.byref(rows), slots.data_ptr(), T, stream))
+
+
+def kv_read(slots: torch.Tensor, cache: KVCache, head_dim: int, *,
+            dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that the codes of ``slots`` (int64 ``[n]``) stand for,
+    ``[n, heads, head_dim]`` each, rounded once to ``dtype``; slots outside the
+    cache read as 0."""
+    dev = _cuda(slots, "slots")
+    _ints(torch.int64, slots=slots)
+    if slots.dim() != 1:
+        raise ValueError(f"slots must be [n], got {tuple(slots.shape)}")
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"dtype must be fp32, fp16 or bf16, got {dtype}")
+    with _Current(dev) as stream:
+        c = _cache_desc(cache, head_dim, dev)
+        n = slots.numel()
+        k = torch.empty((n, cache.k.shape[1], head_dim), dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+        if n:
+            _lib.check(_lib.lib().b200l_kv_read(ctypes.byref(c), slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
+                                                stream))
+    return k, v
+
+
+def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, plan: KVPlan, *,
+                 max_new: int, causal: bool = True, scale: Optional[float] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q K^T) V of new tokens over their requests' cached tokens.
+
+    ``q`` is fp16 or bf16 ``[tokens, query heads, head_dim]`` (contiguous dims),
+    request by request as in ``plan.cu_new``; query head h reads key/value head
+    h // (query heads // cache heads). Of a request with n new tokens of
+    ``seq_lens[r]`` cached ones (int32, the new ones among them), token i sees
+    the keys up to its own position, or all with ``causal=False``. ``max_new``:
+    no request has more new tokens (it chooses the kernel; 1 for a decode step).
+    ``scale`` is head_dim ** -0.5 if not given. A row that sees no key is 0, and
+    so are rows past the plan's tokens. Returns ``out``, contiguous, q's dtype.
+    """
+    dev = _cuda(q, "q")
+    if q.dim() != 3:
+        raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
+    T, hq, dh = q.shape
+    if q.stride(2) != 1 and dh > 1:
+        raise ValueError("q's dims must be contiguous")
+    _on(dev, block_table=block_table, seq_lens=seq_lens, cu_new=plan.cu_new, cu_pages=plan.cu_pages)
+    _ints(torch.int32, seq_lens=seq_lens, cu_new=plan.cu_new, cu_pages=plan.cu_pages)
+    R = seq_lens.numel()
+    if seq_lens.dim() != 1 or plan.cu_new.numel() != R + 1 or plan.cu_pages.numel() != R + 1:
+        raise ValueError(f"seq_lens [requests] and the plan's sums [requests + 1] do not fit: {R}, "
+                         f"{plan.cu_new.numel()}, {plan.cu_pages.numel()}")
+    table_stride = _table_stride(block_table, R)
+    if max_new < 0:
+        raise ValueError(f"max_new must not be negative, got {max_new}")
+    if out is None:
+        out = torch.empty((T, hq, dh), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
+    if T == 0:
+        return out
+    L = _lib.lib()
+    with _Current(dev) as stream:
+        c = _cache_desc(cache, dh, dev)
+        desc = _lib.KVAttnDesc(
+            q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), block_table.data_ptr(),
+            table_stride, seq_lens.data_ptr(), plan.cu_new.data_ptr(),
+            plan.cu_pages.data_ptr(), R, block_table.shape[1], T, hq, max_new, 1 if causal else 0, _DTYPES[q.dtype],
+            dh ** -0.5 if scale is None else scale)
+        need = L.b200l_kv_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(desc))
+        if need == 0:
+            raise _lib.B200LError(-1, _lib.last_error())
+        ws, size = _workspace.get(dev, stream, need)
+        _lib.check(L.b200l_kv_attention(ctypes.byref(c), ctypes.byref(desc), ws, size, stream))
+    return out

@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define B200L_ABI_VERSION 4
+#define B200L_ABI_VERSION 5
 
 enum b200l_status {
     B200L_OK = 0,
@@ -270,6 +270,125 @@ B200L_API int b200l_layer_forward_noalloc(const b200l_layer_desc* desc, const fl
  * or the B200L_ERR_* code a kernel recorded. No counterpart in the reference
  * (see b200l_layer_forward_noalloc). */
 B200L_API int b200l_noalloc_read_status(void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged key/value cache in 8 bits: a causal model's next tokens without its
+ * earlier ones computed again. No counterpart in the reference, which runs
+ * whole sequences only (torch_transformer_benchmark.py:60-123).
+ *
+ * One layer's cache is codes [num_pages, num_heads, page_size, dhp] and fp32
+ * scales [num_pages, num_heads], for K and for V: the tokens of a page share a
+ * scale per head, value = code * scale. dhp is head_dim rounded up to
+ * 32 / 64 / 128 / 256; b200l_kv_append writes the columns past head_dim as
+ * zeros. A slot is page * page_size + place in page. Pages belong to requests:
+ * request r's pages in order are row r of the block table. A step is
+ *   b200l_kv_plan       lengths -> block table, slots of the new tokens   (once)
+ *   b200l_kv_append     new keys and values into their slots         (per layer)
+ *   b200l_kv_attention  new queries over the cache                   (per layer)
+ * Every call is asynchronous on its stream and reads lengths, tables and slots
+ * on the device; page ids and slots outside the cache are passed over.
+ */
+#define B200L_KV_INT8 0  /* code in [-127, 127], scale = max|x| / 127 */
+#define B200L_KV_E4M3 1  /* code an e4m3 float, scale a power of two, max|x| / scale <= 448 */
+#define B200L_KV_MAX_REQUESTS 16384
+
+typedef struct b200l_kv_cache {
+    void* k;              /* codes, 16-byte aligned */
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t num_pages;    /* num_pages * num_heads * page_size < 2^31 */
+    int32_t num_heads;    /* key/value heads */
+    int32_t page_size;    /* tokens of a page: 16, 32, 64 or 128 */
+    int32_t head_dim;     /* 1 .. 256 */
+    int32_t kind;         /* B200L_KV_INT8 or B200L_KV_E4M3 */
+} b200l_kv_cache;
+
+/* Lengths before and after a step -> block table, slots and prefix sums. A
+ * request may grow, stay, or shrink (to 0: finished). Pages are popped from the
+ * top of the stack free_pages[0 .. free_count) by request, then by page; pages
+ * given back are pushed first. What a growing row held is kept; entries past a
+ * shrunken row's pages are stale. Lengths are clamped to [0, table_width *
+ * page_size]. Neither the lengths nor *free_count are changed, and what is read
+ * is not written, so a call repeated gives the same answer; the caller adopts
+ * new_lens and info[0] to go on. With info[1] > 0 pages were missing: their
+ * table entries and slots are -1, and the caller plans again with other
+ * new_lens instead of adopting. */
+typedef struct b200l_kv_plan_desc {
+    const int32_t* old_lens;    /* [requests] */
+    const int32_t* new_lens;    /* [requests] */
+    int32_t* block_table;       /* [requests, table_width], rows table_stride apart; in place */
+    int64_t table_stride;
+    int32_t* free_pages;        /* [capacity] stack; entries from free_count on are written */
+    const int32_t* free_count;  /* [1] */
+    int32_t* cu_new;            /* out [requests + 1]: new tokens, exclusive sums */
+    int32_t* cu_pages;          /* out [requests + 1]: pages of the requests with new tokens, exclusive sums */
+    int32_t* positions;         /* out [max_tokens]: position in its request; -1 past the last new token */
+    int64_t* slots;             /* out [max_tokens]: slot; -1 past the last new token */
+    int32_t* info;              /* out [2]: free pages left, pages missing */
+    int32_t requests;           /* 1 .. B200L_KV_MAX_REQUESTS */
+    int32_t table_width;
+    int32_t page_size;
+    int32_t capacity;
+    int32_t max_tokens;
+} b200l_kv_plan_desc;
+B200L_API int b200l_kv_plan(const b200l_kv_plan_desc* desc, void* stream);
+
+/* New keys and values, [tokens, num_heads, head_dim] with element strides per
+ * token, head and dim. */
+typedef struct b200l_kv_rows {
+    const void* k;
+    const void* v;
+    int64_t k_strides[3];
+    int64_t v_strides[3];
+    int32_t dtype;              /* B200L_DTYPE_F32 / _F16 / _BF16 */
+} b200l_kv_rows;
+
+/* Quantises token i into slots[i] (< 0: not stored). The slots of one page have
+ * to follow one another in the map, as b200l_kv_plan makes them. A page written
+ * from its first place on starts a new scale; else its scale grows to what the
+ * new tokens need and the codes before them are moved to it. A value that is
+ * not finite makes the scale of its page and head not-a-number. */
+B200L_API int b200l_kv_append(const b200l_kv_cache* cache, const b200l_kv_rows* rows, const int64_t* slots,
+                              int64_t tokens, void* stream);
+
+/* The values of n slots, code * scale rounded once to dtype: k_out and v_out
+ * are [n, num_heads, head_dim], contiguous, 16-byte aligned. Slots outside the
+ * cache read as 0. */
+B200L_API int b200l_kv_read(const b200l_kv_cache* cache, const int64_t* slots, int64_t n, void* k_out, void* v_out,
+                            int32_t dtype, void* stream);
+
+/* out = softmax(scale q K^T) V over each request's cached tokens. Token i of
+ * request r (of its n = cu_new[r+1] - cu_new[r]) sees keys [0, seq_lens[r]), or
+ * with causal those up to its own position seq_lens[r] - n + i. Query head h
+ * reads key/value head h / (num_heads / cache heads). A row that sees no key is
+ * 0, as are the rows from cu_new[requests] on. Keys behind block table entries
+ * outside the cache are not there. */
+typedef struct b200l_kv_attn_desc {
+    const void* q;              /* [tokens, num_heads, head_dim], dims contiguous */
+    void* out;                  /* the same shape, contiguous */
+    int64_t q_stride_token;     /* elements */
+    int64_t q_stride_head;
+    const int32_t* block_table;
+    int64_t table_stride;
+    const int32_t* seq_lens;    /* [requests] cached tokens, the new ones among them */
+    const int32_t* cu_new;      /* from b200l_kv_plan */
+    const int32_t* cu_pages;
+    int32_t requests;
+    int32_t table_width;
+    int32_t tokens;
+    int32_t num_heads;          /* query heads, a multiple of the cache's */
+    int32_t max_new;            /* no request has more new tokens */
+    int32_t causal;
+    int32_t dtype;              /* of q and out: B200L_DTYPE_F16 / _BF16 */
+    float scale;
+} b200l_kv_attn_desc;
+
+/* Workspace bytes (1024-byte aligned; status block first: b200l_clear_status
+ * before its first use, b200l_read_status). 0 for a bad shape. */
+B200L_API size_t b200l_kv_attention_workspace_bytes(const b200l_kv_cache* cache, const b200l_kv_attn_desc* desc);
+B200L_API int b200l_kv_attention(const b200l_kv_cache* cache, const b200l_kv_attn_desc* desc, void* workspace,
+                                 size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
