@@ -7,6 +7,7 @@
 #include "kv_common.cuh"
 #include "kv_decode.cuh"
 #include "kv_plan.cuh"
+#include "kv_prompt.cuh"
 
 namespace {
 
@@ -188,7 +189,11 @@ int kv_read_run(const b200l_kv_cache* cache, const int64_t* slots, int64_t n, vo
 // ---------------------------------------------------------------- attention
 struct KvAttnPlan {
   KvAttnArgs a;
-  int dhp, M, workers;
+  int dhp;
+  bool prompt;                   // kv_prompt_kernel; else kv_decode_kernel
+  int M, workers;                // decode: rows of a tile, warps
+  int tiles, splits;             // prompt: row tiles, pieces along the keys
+  long long pieces;              // row tiles that the workspace holds
   size_t off_o, total;
 };
 
@@ -230,21 +235,42 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
   a.causal = d->causal ? 1 : 0;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   a.q_vec = a.q_st % 4 == 0 && a.q_sh % 4 == 0 && !misaligned(d->q, 8);
+  a.q_vec8 = a.q_st % 8 == 0 && a.q_sh % 8 == 0 && !misaligned(d->q, 16);
+  a.o_vec8 = a.dh % 8 == 0 && !misaligned(d->out, 16);
   p->dhp = kv_padded(a.dh);
-  const long long rows = (long long)(d->max_new < d->tokens ? d->max_new : d->tokens) * a.group;
-  p->M = rows > 16 && p->dhp <= 128 ? 32 : 16;
-  const long long tiles = (rows + p->M - 1) / p->M;
-  if (tiles * cache->num_heads > 0x7fffffffLL) return fail(B200L_ERR_BAD_SHAPE, "max_new %d is out of range", d->max_new);
-  a.row_tiles = tiles < 1 ? 1 : (int)tiles;
-  const int tk = p->dhp == 256 ? 16 : p->dhp == 128 ? 32 : 64;
-  a.min_pages = 2 * tk > cache->page_size ? 2 * tk / cache->page_size : 1;
+  if ((long long)d->tokens * a.group > (1ll << 30))
+    return fail(B200L_ERR_BAD_SHAPE, "%d tokens of %d query heads per key head: too many rows", d->tokens, a.group);
+  const int rows = (d->max_new < d->tokens ? d->max_new : d->tokens) * a.group;
   DevInfo dev;
   if ((rc = device_info(&dev))) return rc;
-  p->workers = dev.sms * (p->dhp == 256 || p->M == 32 ? 2 : 3) * 4;
+  // A request's rows fit one or two 16-row tiles of mma.sync, whose kernel is
+  // bound by HBM; beyond, tcgen05's 128-row tiles.
+  p->prompt = rows > 32;
+  if (p->prompt) {
+    const int mq = p->dhp == 256 ? 128 : 256, bn = p->dhp == 256 ? 64 : 128;
+    p->M = mq;
+    p->workers = 0;
+    a.row_tiles = a.min_pages = 0;
+    p->tiles = (int)((long long)d->tokens * a.group / mq) + (d->requests < d->tokens ? d->requests : d->tokens);
+    const long long items = (long long)p->tiles * cache->num_heads;
+    // Few items: as many pieces along the keys as keep every SM busy, of at
+    // least four key tiles each where the table is full.
+    const long long keys = (long long)d->table_width * cache->page_size;
+    const long long most = keys / (4 * bn) > 1 ? keys / (4 * bn) : 1;
+    p->splits = (int)(items >= dev.sms ? 1 : dev.sms / items < most ? dev.sms / items : most);
+    if (items * p->splits > 0x7fffffffLL) return fail(B200L_ERR_BAD_SHAPE, "too many row tiles");
+    p->pieces = p->splits > 1 ? items * p->splits : 0;
+  } else {
+    p->tiles = p->splits = 0;
+    p->M = rows > 16 && p->dhp <= 128 ? 32 : 16;
+    a.row_tiles = rows > p->M ? (rows + p->M - 1) / p->M : 1;
+    const int tk = p->dhp == 256 ? 16 : p->dhp == 128 ? 32 : 64;
+    a.min_pages = 2 * tk > cache->page_size ? 2 * tk / cache->page_size : 1;
+    p->workers = dev.sms * (p->dhp == 256 || p->M == 32 ? 2 : 3) * 4;
+    p->pieces = 2ll * p->workers;
+  }
   p->off_o = 1024;
-  const size_t pieces = (size_t)2 * p->workers * p->M;
-  const size_t off_ml = p->off_o + pieces * p->dhp * 4;
-  p->total = align_up(off_ml + pieces * 8, 1024);
+  p->total = align_up(p->off_o + (size_t)p->pieces * p->M * (p->dhp + 2) * 4, 1024);
   a.part_o = nullptr;
   a.part_ml = nullptr;
   return B200L_OK;
@@ -273,6 +299,42 @@ int kv_decode_t(KvAttnPlan& p, uint8_t* ws, cudaStream_t st) {
   return check_launch("kv_join_kernel");
 }
 
+template <int DHP, int KIND>
+int kv_prompt_t(const KvAttnPlan& p, uint8_t* ws, cudaStream_t st) {
+  using C = KvPromptCfg<DHP>;
+  auto kern = kv_prompt_kernel<DHP, KIND>;
+  int rc = ensure_smem((const void*)kern, C::SMEM);
+  if (rc) return rc;
+  if (C::NQ == 2) {
+    // The warps share out the registers of the launch: fewer than planned for, and they would wait for ever.
+    static std::atomic<int> regs{0};
+    if (!regs.load()) {
+      cudaFuncAttributes fa;
+      cudaError_t e = cudaFuncGetAttributes(&fa, (const void*)kern);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(kv_prompt_kernel)");
+      regs.store(fa.numRegs);
+    }
+    if (regs.load() < C::R_LAUNCH)
+      return fail(B200L_ERR_LAUNCH, "kv_prompt_kernel was built with %d registers, its shares need %d", regs.load(), C::R_LAUNCH);
+  }
+  DevInfo dev;
+  if ((rc = device_info(&dev))) return rc;
+  KvPromptArgs pa;
+  pa.a = p.a;
+  pa.tiles = p.tiles;
+  pa.splits = p.splits;
+  pa.min_rows = 1;
+  const long long items = (long long)p.tiles * p.a.c.heads * p.splits;
+  const int grid = (int)(items < dev.sms ? items : dev.sms);
+  cudaError_t e = launch_pdl(kern, dim3(grid), dim3(C::THREADS), C::SMEM, st, pa, reinterpret_cast<DevStatus*>(ws));
+  if (e != cudaSuccess) return cuda_fail(e, "kv_prompt_kernel");
+  if ((rc = check_launch("kv_prompt_kernel"))) return rc;
+  if (p.splits == 1) return B200L_OK;
+  e = launch_pdl(kv_prompt_join_kernel<DHP>, dim3(p.tiles * p.a.c.heads, 8), dim3(256), 0, st, pa);
+  if (e != cudaSuccess) return cuda_fail(e, "kv_prompt_join_kernel");
+  return check_launch("kv_prompt_join_kernel");
+}
+
 int kv_attention_run(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, void* ws, size_t ws_bytes, cudaStream_t st) {
   KvAttnPlan p;
   int rc = kv_attn_plan(cache, d, &p);
@@ -286,7 +348,12 @@ int kv_attention_run(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, v
   if (ws_bytes < p.total) return fail(B200L_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", ws_bytes, p.total);
   uint8_t* w = static_cast<uint8_t*>(ws);
   p.a.part_o = reinterpret_cast<float*>(w + p.off_o);
-  p.a.part_ml = p.a.part_o + (size_t)2 * p.workers * p.M * p.dhp;
+  p.a.part_ml = p.a.part_o + (size_t)p.pieces * p.M * p.dhp;
+  if (p.prompt) {
+#define KV_CALL(D, K) kv_prompt_t<D, K>(p, w, st)
+    KV_DISPATCH(cache->head_dim, cache->kind, KV_CALL)
+#undef KV_CALL
+  }
   if (p.M == 32) {
     switch (p.dhp * 2 + cache->kind) {
       case 64: return kv_decode_t<32, kKvInt8, 2>(p, w, st);

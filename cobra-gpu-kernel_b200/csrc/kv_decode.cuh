@@ -48,7 +48,7 @@ struct KvAttnArgs {
   const int* cu_pages;
   float* part_o;                 // [2 * workers][M][dhp]
   float* part_ml;                // [2 * workers][M][2]
-  int requests, width, tokens, hq, group, dh, type, causal, row_tiles, min_pages, q_vec;
+  int requests, width, tokens, hq, group, dh, type, causal, row_tiles, min_pages, q_vec, q_vec8, o_vec8;
   float scale_log2;              // softmax scale * log2(e)
 };
 

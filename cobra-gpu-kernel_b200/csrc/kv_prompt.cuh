@@ -1,0 +1,682 @@
+// kv_prompt.cuh -- attention of many rows per request over a paged 8-bit cache:
+// prompt chunks, whole prompts, long guesses.
+//
+// Same definition as kv_decode.cuh. A work item is (request, key head, 256 rows
+// = two tiles of 128 that share every K / V tile; 128 rows at dhp 256), a row
+// being one query head of one new token; items of few requests are cut along
+// the keys as well, and kv_prompt_join_kernel adds the pieces in order.
+//
+// tcgen05 multiplies fp16, so codes become fp16 (exactly) on their way: bulk
+// copies bring a tile's pages as they lie into shared memory, four warps turn
+// them into swizzled fp16 rows (K as the K-major operand of S = Q K^T, V as the
+// MN-major one of O += P V, the same layout), and the scales stay out of the
+// products: per 16 keys, one page's worth at least, the softmax has c = scale
+// log2(e) s_k, log2 s_v and 1 / s_v, so that u = c s + log2 s_v is the one fused
+// multiply-add that the exponent needs anyway, the row maximum is taken per 16
+// raw scores (c >= 0) and the row sum is corrected once per 16 weights.
+//
+// Warps: 0 loads pages and scales, 1 issues S of both tiles, 2 / 3 issue P V of
+// tile 0 / 1, 4-7 convert, 8.. are the softmax (eight per tile, 16 rows a warp,
+// two threads per row with half the keys each). P goes back to TMEM as fp16: in
+// its own columns where they suffice (dhp <= 64, and dhp 256 with one tile), so
+// that the next S is computed meanwhile; over S at dhp 128, where two O and two
+// S fill TMEM and the tiles alternate instead. O is rescaled only when a row's
+// maximum grew by 2^8.
+//
+// Bound: exponentials and products alike at dhp 128 (16 per clock and SM, 2048
+// clocks a 256 x 128 tile, and 4 x 512 clocks of tcgen05), exponentials below.
+#pragma once
+
+#include "kv_decode.cuh"
+
+namespace b200l {
+
+struct KvPromptArgs {
+  KvAttnArgs a;                  // part_o / part_ml: [items][splits][rows]([dhp])
+  int tiles;                     // row tiles of all requests, at most
+  int splits;                    // pieces along the keys
+  int min_rows;                  // requests with fewer rows are the decode kernel's
+};
+
+template <int DHP>
+struct KvPromptCfg {
+  static constexpr int NQ = DHP == 256 ? 1 : 2;             // query tiles of an item
+  static constexpr int MQ = NQ * 128;
+  static constexpr int BN = DHP == 256 ? 64 : 128;          // keys of a tile
+  static constexpr int ROWB = DHP == 32 ? 64 : 128;         // bytes of a swizzled fp16 row
+  static constexpr int NH = DHP * 2 / ROWB;                 // such rows side by side
+  static constexpr int Q_BYTES = 128 * DHP * 2;
+  static constexpr int KV_BYTES = BN * DHP * 2;             // an fp16 tile of K or V
+  static constexpr int C_BYTES = BN * DHP;                  // its codes
+  static constexpr int ST8 = DHP <= 64 ? 2 : 1;             // stages of codes
+  static constexpr bool OVER = DHP == 128;                  // P overwrites S
+  static constexpr int GR = BN / 16;                        // 16-key groups of a tile
+  static constexpr int CSLOTS = 8;                          // stages of their constants
+  static constexpr int SM_CONST = CSLOTS * (GR + 1) * 16;
+  static constexpr int SMEM = NQ * Q_BYTES + 4 * KV_BYTES + ST8 * 2 * C_BYTES + SM_CONST + 48 * 8 + 1024;
+  static constexpr int SOFT = NQ * 8;                       // softmax warps
+  static constexpr int THREADS = 256 + 32 * SOFT;
+  static constexpr int S_COL = 0;                           // + 128 t
+  static constexpr int P_COL = OVER ? 0 : DHP == 256 ? 64 : 256;
+  static constexpr int P_STEP = OVER ? 128 : 64;
+  static constexpr int O_COL = DHP <= 64 ? 384 : 256;
+  static constexpr int O_STEP = DHP <= 64 ? 64 : 128;
+  // Registers of the three kinds of warps (setmaxnreg); together what the
+  // launch holds: 768 threads of 80.
+  static constexpr int R_LAUNCH = 80, R_ISSUE = 40, R_CONV = 56, R_SOFT = 96;
+};
+static_assert(128 * (KvPromptCfg<128>::R_ISSUE + KvPromptCfg<128>::R_CONV) + 512 * KvPromptCfg<128>::R_SOFT ==
+                  768 * KvPromptCfg<128>::R_LAUNCH,
+              "the register shares add up to the launch's");
+
+// A work item: rows [row0, row0 + MQ) of request r for key head h, key tiles [j0, j1).
+struct KvItem {
+  int r, h, row0, rows, n, len, tok0, nqt, j0, j1, piece;
+};
+
+template <int DHP>
+__device__ __forceinline__ bool kv_item(const KvPromptArgs& p, int item, int lane, KvItem& it) {
+  using C = KvPromptCfg<DHP>;
+  const KvAttnArgs& a = p.a;
+  it.piece = item % p.splits;
+  const int xh = item / p.splits;
+  it.h = xh % a.c.heads;
+  const int x = p.tiles - 1 - xh / a.c.heads;     // the last rows see the most keys: first
+  // Request r's tiles begin at floor(cu_new[r] group / MQ) + min(r, cu_new[r]):
+  // room for every request with new tokens; what is left over is skipped.
+  int lo = 0, hi = a.requests;
+  auto base = [&](int r) { return (int)((long long)a.cu_new[r] * a.group / C::MQ) + min(r, a.cu_new[r]); };
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+    const int k = __popc(__ballot_sync(0xffffffffu, at < hi && base(at) <= x));
+    hi = min(hi, lo + (k + 1) * step);
+    lo += k * step;
+  }
+  it.r = lo;
+  it.tok0 = a.cu_new[lo];
+  it.n = a.cu_new[lo + 1] - it.tok0;
+  it.rows = it.n * a.group;
+  it.row0 = (x - base(lo)) * C::MQ;
+  if (it.row0 < 0 || it.row0 >= it.rows || it.rows < p.min_rows) return false;
+  it.nqt = it.rows - it.row0 > 128 && C::NQ == 2 ? 2 : 1;
+  it.len = min(max(a.lens[lo], 0), min(a.cu_pages[lo + 1] - a.cu_pages[lo], a.width) << a.c.log2_page);
+  const int last = min(it.row0 + C::MQ, it.rows) - 1;
+  const int end = a.causal ? min(it.len, max(0, it.len - it.n + last / a.group + 1)) : it.len;
+  const int nt = (end + C::BN - 1) / C::BN;
+  it.j0 = (int)((long long)nt * it.piece / p.splits);
+  it.j1 = (int)((long long)nt * (it.piece + 1) / p.splits);
+  return true;
+}
+
+// Shared-memory descriptor of an MN-major B operand: K rows of ROWB bytes, 8 of
+// them a swizzle atom, atoms SBO = 8 ROWB apart along K and LBO along N.
+__device__ __forceinline__ uint64_t sdesc_mnmajor(uint32_t saddr, int row_bytes, uint32_t lbo) {
+  uint64_t d = sdesc_kmajor(saddr, row_bytes);
+  d &= ~(uint64_t(0x3fff) << 16);
+  return d | (uint64_t)((lbo >> 4) & 0x3fff) << 16;
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int DHP, int KIND>
+__global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel(KvPromptArgs p, DevStatus* status) {
+  using C = KvPromptCfg<DHP>;
+  constexpr int BN = C::BN, GR = C::GR, HC = BN / 2;
+  const KvAttnArgs& a = p.a;
+  pdl_wait_then_release();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + C::NQ * C::Q_BYTES;
+  uint8_t* sV = sK + 2 * C::KV_BYTES;
+  uint8_t* c8K = sV + 2 * C::KV_BYTES;
+  uint8_t* c8V = c8K + C::ST8 * C::C_BYTES;
+  float4* consts = reinterpret_cast<float4*>(c8V + C::ST8 * C::C_BYTES);   // [CSLOTS][GR + 1]; the last: .x = whole
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(consts) + C::SM_CONST);
+  uint64_t* q_full = bars;          // [2]
+  uint64_t* q_empty = bars + 2;     // [2]
+  uint64_t* k8_full = bars + 4;     // [2]
+  uint64_t* k8_free = bars + 6;     // [2]
+  uint64_t* v8_full = bars + 8;     // [2]
+  uint64_t* v8_free = bars + 10;    // [2]
+  uint64_t* k_full = bars + 12;     // [2]
+  uint64_t* k_empty = bars + 14;    // [2]
+  uint64_t* v_full = bars + 16;     // [2]
+  uint64_t* v_empty = bars + 18;    // [2]
+  uint64_t* s_full = bars + 20;     // [2]
+  uint64_t* s_free = bars + 22;     // [2]
+  uint64_t* p_full = bars + 24;     // [2]
+  uint64_t* pv_done = bars + 26;    // [2]
+  uint64_t* c_full = bars + 28;     // [CSLOTS]
+  uint64_t* mma_done = bars + 36;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 37);
+  WaitCtl* wc = reinterpret_cast<WaitCtl*>(bars + 38);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 8);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&k8_full[i], 1);
+      mbar_init(&k8_free[i], 4);
+      mbar_init(&v8_full[i], 1);
+      mbar_init(&v8_free[i], 4);
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], C::NQ);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 8);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < C::CSLOTS; ++i) mbar_init(&c_full[i], 1);
+    mbar_init(mma_done, 1 + C::NQ);
+    waitctl_init(wc, status);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int items = p.tiles * a.c.heads * p.splits;
+  const int P = a.c.page, lp = a.c.log2_page, PB = P < BN ? P : BN;
+
+  if (warp < 4) {
+    if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_ISSUE));
+    if (warp == 0) {  // ================= pages and scales
+      int g = 0, gk = 0, gv = 0;                  // tiles; K and V copies begun
+      bool ok = true;
+      KvItem it;
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        if (!kv_item<DHP>(p, item, lane, it)) continue;
+        const int* row = a.table + it.r * a.table_stride;
+        auto entry_at = [&](int j) {              // page of this lane's part of key tile j
+          const int k = j * BN + lane * PB;
+          return (lane * PB < BN && k < it.len && (k >> lp) < a.width) ? row[k >> lp] : -1;
+        };
+        int next = it.j0 < it.j1 ? entry_at(it.j0) : -1;
+        for (int j = it.j0; j < it.j1; ++j, ++g) {
+          const int s8 = g % C::ST8, cs = g % C::CSLOTS, id = next;
+          if (j + 1 < it.j1) next = entry_at(j + 1);
+          const bool there = id >= 0 && id < a.c.num_pages;
+          const long long ph = there ? (long long)id * a.c.heads + it.h : 0;
+          const float sk = there ? a.c.k_scale[ph] : 0.f, sv = there ? a.c.v_scale[ph] : 0.f;
+          const long long src = ((ph << lp) + ((j * BN + lane * PB) & (P - 1))) * DHP;
+          const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, there));
+          const uint32_t parity = ((g / C::ST8) & 1) ^ 1;
+          if (!mbar_wait_warp(&k8_free[s8], parity, wc)) { ok = false; break; }
+          if (lane == 0) mbar_arrive_expect_tx(&k8_full[s8], boxes * (uint32_t)(PB * DHP));
+          __syncwarp();
+          if (there) bulk_load(c8K + s8 * C::C_BYTES + lane * PB * DHP, a.c.k + src, PB * DHP, &k8_full[s8]);
+          ++gk;
+          // The constants of this lane's keys, 16 at a time.
+          if (lane * PB < BN) {
+            const float svc = fmaxf(sv, 7.8886090522101181e-31f);      // 2^-100 for a page of zeros
+            float4 c;
+            c.x = sk;
+            c.y = !there ? -INFINITY : sv == sv ? __log2f(svc) : sv;
+            c.z = !there || !(svc < INFINITY) ? 0.f : __fdividef(1.0f, svc);
+            c.w = there ? 1.f : 0.f;
+            for (int i = 0; i < PB / 16; ++i) consts[cs * (GR + 1) + lane * (PB / 16) + i] = c;
+          }
+          const int want = min(BN / PB, (it.len - j * BN + PB - 1) / PB);
+          if (lane == 0) consts[cs * (GR + 1) + GR].x = (int)boxes >= want && (j + 1) * BN <= it.len ? 1.f : 0.f;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&c_full[cs]);
+          if (!mbar_wait_warp(&v8_free[s8], parity, wc)) { ok = false; break; }
+          if (lane == 0) mbar_arrive_expect_tx(&v8_full[s8], boxes * (uint32_t)(PB * DHP));
+          __syncwarp();
+          if (there) bulk_load(c8V + s8 * C::C_BYTES + lane * PB * DHP, a.c.v + src, PB * DHP, &v8_full[s8]);
+          ++gv;
+        }
+      }
+      // Copies in flight land before the block goes (each stage's last one).
+      for (int i = max(0, gk - C::ST8); i < gk; ++i) mbar_drain(&k8_full[i % C::ST8], (i / C::ST8) & 1);
+      for (int i = max(0, gv - C::ST8); i < gv; ++i) mbar_drain(&v8_full[i % C::ST8], (i / C::ST8) & 1);
+    } else if (warp == 1) {  // ================= S_t(j) = Q_t K_j^T
+      const uint32_t idesc_s = idesc_f16_f32(128, BN);
+      const uint64_t dq0 = sdesc_kmajor(smem_u32(sQ), C::ROWB);
+      const uint64_t dk0 = sdesc_kmajor(smem_u32(sK), C::ROWB);
+      int g = 0, ns[2] = {0, 0}, qi[2] = {0, 0};
+      bool ok = true;
+      KvItem it;
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        if (!kv_item<DHP>(p, item, lane, it) || it.j0 >= it.j1) continue;
+        if (lane == 0) {
+          for (int t = 0; t < it.nqt && ok; ++t) ok = mbar_wait(&q_full[t], qi[t]++ & 1, wc);
+          for (int j = it.j0; j < it.j1 && ok; ++j, ++g) {
+            const int st = g & 1;
+            if (!mbar_wait(&k_full[st], (g >> 1) & 1, wc)) { ok = false; break; }
+            const uint64_t dk = dk0 + (uint64_t)((st * C::KV_BYTES) >> 4);
+            for (int t = 0; t < it.nqt; ++t) {
+              // S_t's columns are free once the softmax has read them; where P
+              // takes their place, once P V has read that.
+              if (ns[t] > 0 && !mbar_wait(C::OVER ? &pv_done[t] : &s_free[t], (ns[t] - 1) & 1, wc)) { ok = false; break; }
+              const uint64_t dq = dq0 + (uint64_t)((t * C::Q_BYTES) >> 4);
+              const uint32_t d_s = tmem_base + C::S_COL + t * 128;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < DHP / 16; ++k) {
+                constexpr int R = C::ROWB;
+                const uint32_t off_q = (uint32_t)((k * 32) / R) * (128 * R) + (k * 32) % R;
+                const uint32_t off_k = (uint32_t)((k * 32) / R) * (BN * R) + (k * 32) % R;
+                umma_f16_ss(d_s, dq + (off_q >> 4), dk + (off_k >> 4), idesc_s, k > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[t]);
+              ++ns[t];
+            }
+            if (ok) umma_commit(&k_empty[st]);
+          }
+          if (ok)
+            for (int t = 0; t < it.nqt; ++t) umma_commit(&q_empty[t]);
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      }
+      if (lane == 0) {
+        umma_commit(mma_done);
+        mbar_drain(mma_done, 0);
+      }
+    } else if (warp - 2 < C::NQ) {  // ================= O_t += P_t(j) V_j
+      const int t = warp - 2;
+      const uint32_t idesc_o = idesc_f16_f32(128, DHP) | (1u << 16);       // B is MN-major
+      const uint64_t dv0 = sdesc_mnmajor(smem_u32(sV), C::ROWB, BN * C::ROWB);
+      const uint32_t a_p = tmem_base + C::P_COL + t * C::P_STEP;
+      const uint32_t d_o = tmem_base + C::O_COL + t * C::O_STEP;
+      int g = 0, np = 0;
+      bool ok = true;
+      KvItem it;
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        if (!kv_item<DHP>(p, item, lane, it) || it.j0 >= it.j1) continue;
+        if (lane == 0) {
+          for (int j = it.j0; j < it.j1 && ok; ++j, ++g) {
+            const int st = g & 1;
+            if (!mbar_wait(&v_full[st], (g >> 1) & 1, wc)) { ok = false; break; }
+            if (t >= it.nqt) {                    // no second tile: the stage is released as it comes
+              umma_commit(&v_empty[st]);
+              continue;
+            }
+            if (!mbar_wait(&p_full[t], np & 1, wc)) { ok = false; break; }
+            const uint64_t dv = dv0 + (uint64_t)((st * C::KV_BYTES) >> 4);
+            const uint32_t acc0 = j > it.j0 ? 1u : 0u;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              umma_f16_ts(d_o, a_p + k * 8, dv + ((uint32_t)(k * 16 * C::ROWB) >> 4), idesc_o, k > 0 ? 1u : acc0);
+            umma_commit(&pv_done[t]);
+            umma_commit(&v_empty[st]);
+            ++np;
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      }
+      if (lane == 0) {
+        umma_commit(mma_done);
+        mbar_drain(mma_done, 0);
+      }
+    }
+  } else if (warp < 8) {  // ================= codes -> fp16
+    if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_CONV));
+    const int tid = threadIdx.x - 128;
+    constexpr int UPR = DHP / 16;                 // 16-code pieces of a row
+    constexpr int UNITS = BN * UPR / 128;         // ... of a thread
+    constexpr int UPH = C::ROWB / 32;             // ... of a swizzled fp16 row
+    int g = 0;
+    bool ok = true;
+    KvItem it;
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      if (!kv_item<DHP>(p, item, lane, it)) continue;
+      for (int j = it.j0; j < it.j1 && ok; ++j, ++g) {
+        const int s8 = g % C::ST8, cs = g % C::CSLOTS, st = g & 1;
+        if (!mbar_wait_warp(&c_full[cs], (g / C::CSLOTS) & 1, wc)) { ok = false; break; }
+        const float4* cc = consts + cs * (GR + 1);
+        const bool whole = cc[GR].x != 0.f;
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+          uint64_t* full8 = which ? &v8_full[s8] : &k8_full[s8];
+          uint64_t* free8 = which ? &v8_free[s8] : &k8_free[s8];
+          uint64_t* full = which ? &v_full[st] : &k_full[st];
+          uint64_t* empty = which ? &v_empty[st] : &k_empty[st];
+          const uint8_t* src = (which ? c8V : c8K) + s8 * C::C_BYTES;
+          const uint32_t dst = smem_u32((which ? sV : sK) + st * C::KV_BYTES);
+          if (!mbar_wait_warp(full8, (g / C::ST8) & 1, wc) || !mbar_wait_warp(empty, ((g >> 1) & 1) ^ 1, wc)) {
+            ok = false;
+            break;
+          }
+          constexpr int BATCH = UNITS < 4 ? UNITS : 4;
+#pragma unroll 1
+          for (int u0 = 0; u0 < UNITS; u0 += BATCH) {
+            uint4 w[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) w[i] = *reinterpret_cast<const uint4*>(src + ((u0 + i) * 128 + tid) * 16);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+              const int unit = (u0 + i) * 128 + tid, row = unit / UPR, c16 = unit % UPR;
+              // What lies past the keys, or in a page that is not there, is no number.
+              if (!whole && (j * BN + row >= it.len || cc[row >> 4].w == 0.f)) w[i] = make_uint4(0, 0, 0, 0);
+              uint32_t h[8];
+              codes4_to_half<KIND>(w[i].x, h[0], h[1]);
+              codes4_to_half<KIND>(w[i].y, h[2], h[3]);
+              codes4_to_half<KIND>(w[i].z, h[4], h[5]);
+              codes4_to_half<KIND>(w[i].w, h[6], h[7]);
+              const int hb = c16 / UPH, ch = 2 * (c16 % UPH), odd = hb & 1;
+              const uint32_t base = dst + hb * BN * C::ROWB;
+              // (neighbouring halves write their odd pieces first: no bank conflicts)
+              st_shared_v4(base + swz_offset(row, ch + odd, C::ROWB), odd ? h[4] : h[0], odd ? h[5] : h[1], odd ? h[6] : h[2],
+                           odd ? h[7] : h[3]);
+              st_shared_v4(base + swz_offset(row, ch + 1 - odd, C::ROWB), odd ? h[0] : h[4], odd ? h[1] : h[5],
+                           odd ? h[2] : h[6], odd ? h[3] : h[7]);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(full);
+            mbar_arrive(free8);
+          }
+        }
+      }
+    }
+  } else {  // ================= softmax
+    if constexpr (C::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFT));
+    const int sw = warp - 8, t = sw >> 3, hh = (sw >> 2) & 1, qd = warp & 3;
+    const int c = lane >> 4;                      // key half, and dim half, of this thread
+    const int row = qd * 32 + hh * 16 + (lane & 15);
+    const uint32_t lane_off = (uint32_t)(qd * 32 + hh * 16) << 16;
+    const uint32_t t_s = tmem_base + lane_off + C::S_COL + t * 128;
+    const uint32_t t_p = tmem_base + lane_off + C::P_COL + t * C::P_STEP;
+    const uint32_t t_o = tmem_base + lane_off + C::O_COL + t * C::O_STEP;
+    constexpr int OH = DHP / 2;                   // dims of this thread
+    constexpr int OC = OH < 32 ? OH : 32;         // ... at a time
+    int g = 0, ns = 0, np = 0, qi = 0;
+    bool ok = true;
+    // Rows past the plan's tokens.
+    for (long long i = (long long)a.cu_new[a.requests] * a.hq * a.dh + (blockIdx.x * C::SOFT + sw) * 32 + lane,
+                   e = (long long)a.tokens * a.hq * a.dh;
+         i < e; i += (long long)gridDim.x * C::SOFT * 32)
+      static_cast<unsigned short*>(a.out)[i] = 0;
+    KvItem it;
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      if (!kv_item<DHP>(p, item, lane, it)) continue;
+      if (t >= it.nqt) {
+        g += it.j1 - it.j0;
+        continue;
+      }
+      const int gr = it.row0 + t * 128 + row, i = gr / a.group, hq = it.h * a.group + gr - i * a.group;
+      const bool in = gr < it.rows && it.tok0 + i < a.tokens;
+      const int lim = !in ? 0 : a.causal ? min(it.len, it.len - it.n + i + 1) : it.len;
+      const int first = (it.row0 + t * 128) / a.group;              // the tile's first token sees least
+      const int lim_min = a.causal ? min(it.len, it.len - it.n + first + 1) : it.len;
+      float qs = a.scale_log2, m_use = 0.f, l = 0.f;
+      bool none = true;                           // no visible key so far
+      if (it.j0 < it.j1) {  // ---- Q_t as fp16, scaled by a power of two if it comes as bf16
+        const long long at = (long long)(it.tok0 + i) * a.q_st + (long long)hq * a.q_sh + c * OH;
+        uint32_t w[OH / 2];
+        if (in && a.q_vec8 && (c + 1) * OH <= a.dh) {
+#pragma unroll
+          for (int d = 0; d < OH / 8; ++d) {
+            const uint4 u = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + at)[d];
+            w[4 * d] = u.x;
+            w[4 * d + 1] = u.y;
+            w[4 * d + 2] = u.z;
+            w[4 * d + 3] = u.w;
+          }
+        } else {
+          const unsigned short* q = static_cast<const unsigned short*>(a.q) + at;
+#pragma unroll
+          for (int d = 0; d < OH / 2; ++d) {
+            const int d0 = c * OH + 2 * d;
+            const uint32_t x = in && d0 < a.dh ? q[2 * d] : 0u, y = in && d0 + 1 < a.dh ? q[2 * d + 1] : 0u;
+            w[d] = x | y << 16;
+          }
+        }
+        if (a.type == kElemBF16) {
+          float big = 0.f;
+#pragma unroll
+          for (int d = 0; d < OH / 2; ++d) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[d]));
+            big = fmax3f(big, fabsf(f.x), fabsf(f.y));
+          }
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
+          float mul = 1.f;
+          if (big > 0.f && big < INFINITY) {
+            const int ex = min(max(((__float_as_int(big) >> 23) & 255) - 127, -120), 120);
+            mul = __int_as_float((127 - ex) << 23);
+            qs *= __int_as_float((127 + ex) << 23);
+          }
+#pragma unroll
+          for (int d = 0; d < OH / 2; ++d) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[d]));
+            w[d] = pack_half2(f.x * mul, f.y * mul);
+          }
+        }
+        if (!mbar_wait_warp(&q_empty[t], (qi & 1) ^ 1, wc)) { ok = false; break; }
+        ++qi;
+        const uint32_t dst = smem_u32(sQ + t * C::Q_BYTES);
+#pragma unroll
+        for (int d = 0; d < OH / 8; ++d) {
+          const int chunk = c * (OH / 8) + d;     // 8 dims
+          st_shared_v4(dst + (chunk / (C::ROWB / 16)) * 128 * C::ROWB + swz_offset(row, chunk % (C::ROWB / 16), C::ROWB),
+                       w[4 * d], w[4 * d + 1], w[4 * d + 2], w[4 * d + 3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[t]);
+      }
+      for (int j = it.j0; j < it.j1; ++j, ++g) {
+        const int cs = g % C::CSLOTS;
+        if (!mbar_wait_warp(&c_full[cs], (g / C::CSLOTS) & 1, wc) || !mbar_wait_warp(&s_full[t], ns & 1, wc)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float s[HC];
+        {
+          uint32_t r[HC];
+          tmem_ld_pair32<HC>(t_s, *reinterpret_cast<uint32_t(*)[32]>(r));
+          if constexpr (HC == 64) tmem_ld_pair32<HC>(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+#pragma unroll
+          for (int k = 0; k < HC; ++k) s[k] = __uint_as_float(r[k]);
+        }
+        tc_fence_before();
+        if constexpr (!C::OVER) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[t]);
+        }
+        ++ns;
+        const int kv0 = j * BN + HC * c;          // first key of this thread's half
+        const bool edge = (j + 1) * BN > lim_min; // (warp-uniform)
+        if (edge) {
+#pragma unroll
+          for (int k = 0; k < HC; ++k)
+            if (kv0 + k >= lim) s[k] = -INFINITY;
+        }
+        const float4* cc = consts + cs * (GR + 1) + c * (GR / 2);
+        float cg[HC / 16], lg[HC / 16], ig[HC / 16], hm = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < HC / 16; ++q) {
+          const float4 k4 = cc[q];
+          cg[q] = k4.x * qs;
+          lg[q] = k4.y;
+          ig[q] = k4.z;
+          float m0 = fmaxf(s[16 * q], s[16 * q + 1]), m1 = fmaxf(s[16 * q + 2], s[16 * q + 3]);
+#pragma unroll
+          for (int k = 4; k < 16; k += 4) {
+            m0 = fmax3f(m0, s[16 * q + k], s[16 * q + k + 1]);
+            m1 = fmax3f(m1, s[16 * q + k + 2], s[16 * q + k + 3]);
+          }
+          hm = fmaxf(hm, fmaf(fmaxf(m0, m1), cg[q], lg[q]));
+        }
+        const float m_cand = fmaxf(hm, __shfl_xor_sync(0xffffffffu, hm, 16));
+        float alpha = 1.f;
+        bool rescale = false;
+        if (none) {
+          if (m_cand > -INFINITY) {
+            none = false;
+            m_use = m_cand;
+          }
+        } else if (m_cand > m_use + 8.f) {
+          alpha = ex2_approx(m_use - m_cand);
+          m_use = m_cand;
+          rescale = true;
+        }
+        float sum = 0.f;
+        uint32_t pk[HC / 2];
+#pragma unroll
+        for (int q = 0; q < HC / 16; ++q) {
+          const float lm = lg[q] - m_use;
+          const float2 c2 = make_float2(cg[q], cg[q]), l2 = make_float2(lm, lm);
+          float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float2 x = __ffma2_rn(make_float2(s[16 * q + 2 * k], s[16 * q + 2 * k + 1]), c2, l2);
+            if (edge) {                           // (a factor of 0 or not-a-number does not bring hidden keys back)
+              if (kv0 + 16 * q + 2 * k >= lim) x.x = -INFINITY;
+              if (kv0 + 16 * q + 2 * k + 1 >= lim) x.y = -INFINITY;
+            }
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            if (k & 1) a1 = __fadd2_rn(a1, e);
+            else a0 = __fadd2_rn(a0, e);
+            pk[8 * q + k] = pack_half2(e.x, e.y);
+          }
+          const float2 as = __fadd2_rn(a0, a1);
+          sum = fmaf(as.x + as.y, ig[q], sum);
+        }
+        l = fmaf(l, alpha, sum);
+        if (np > 0) {                             // P and O are free once the last P V is done
+          if (!mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc)) { ok = false; break; }
+          tc_fence_after();
+        }
+        if (j > it.j0 && __any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+          for (int d = 0; d < OH / OC; ++d) {
+            uint32_t r[OC];
+            if constexpr (OC == 16) tmem_ld_pair16<OH>(t_o, *reinterpret_cast<uint32_t(*)[16]>(r));
+            else tmem_ld_pair32<OH>(t_o + d * OC, *reinterpret_cast<uint32_t(*)[32]>(r));
+#pragma unroll
+            for (int k = 0; k < OC; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+            if constexpr (OC == 16) tmem_st_pair16<OH>(t_o, *reinterpret_cast<uint32_t(*)[16]>(r));
+            else tmem_st_pair32<OH>(t_o + d * OC, *reinterpret_cast<uint32_t(*)[32]>(r));
+          }
+        }
+        if constexpr (HC == 64) tmem_st_pair32<32>(t_p, *reinterpret_cast<uint32_t(*)[32]>(pk));
+        else tmem_st_pair16<16>(t_p, *reinterpret_cast<uint32_t(*)[16]>(pk));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+        ++np;
+      }
+      if (!ok) break;
+      // ---- the rows' results, or this piece of them
+      const bool any = it.j0 < it.j1;
+      if (any) {
+        if (!mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc)) { ok = false; break; }
+        tc_fence_after();
+      }
+      const float lt = l + __shfl_xor_sync(0xffffffffu, l, 16);
+      const float r1 = lt == 0.f ? 0.f : 1.0f / lt;
+      const long long xh = item / p.splits;
+      const long long pr = (xh * p.splits + it.piece) * C::MQ + t * 128 + row;
+      if (p.splits > 1 && in && c == 0) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(none ? -INFINITY : m_use, lt);
+      const long long oat = ((long long)(it.tok0 + i) * a.hq + hq) * a.dh;
+#pragma unroll
+      for (int d = 0; d < OH / OC; ++d) {
+        uint32_t r[OC];
+        if (any) {
+          if constexpr (OC == 16) tmem_ld_pair16<OH>(t_o, *reinterpret_cast<uint32_t(*)[16]>(r));
+          else tmem_ld_pair32<OH>(t_o + d * OC, *reinterpret_cast<uint32_t(*)[32]>(r));
+        } else {
+#pragma unroll
+          for (int k = 0; k < OC; ++k) r[k] = 0u;
+        }
+        const int d0 = c * OH + d * OC;
+        if (in) {
+          if (p.splits > 1) {
+            float4* o = reinterpret_cast<float4*>(a.part_o + pr * DHP + d0);
+#pragma unroll
+            for (int k = 0; k < OC / 4; ++k)
+              o[k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]), __uint_as_float(r[4 * k + 2]),
+                                 __uint_as_float(r[4 * k + 3]));
+          } else if (a.o_vec8 && d0 + OC <= a.dh) {
+            uint4* o = reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + oat + d0);
+#pragma unroll
+            for (int k = 0; k < OC / 8; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_elem2(__uint_as_float(r[8 * k + 2 * e]) * r1, __uint_as_float(r[8 * k + 2 * e + 1]) * r1, a.type);
+              o[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < OC; k += 2)
+              if (d0 + k < a.dh) store_out(a, oat, d0 + k, __uint_as_float(r[k]) * r1, __uint_as_float(r[k + 1]) * r1);
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && waitctl_aborted(wc)) record_error(status, -7, kKernelKvPrompt, 1);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Adds the pieces of each row in order; a warp per row, the rows of an item
+// spread over blocks.
+template <int DHP>
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(KvPromptArgs p) {
+  pdl_wait_then_release();
+  using C = KvPromptCfg<DHP>;
+  const KvAttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  KvItem it;
+  const int item = blockIdx.x * p.splits;         // (its first piece)
+  if (!kv_item<DHP>(p, item, lane, it)) return;
+  for (int row = blockIdx.y * 8 + warp; row < C::MQ; row += gridDim.y * 8) {
+    const int gr = it.row0 + row, i = gr / a.group;
+    if (gr >= it.rows || it.tok0 + i >= a.tokens) break;
+    const long long at = (long long)item * C::MQ + row;              // + piece * MQ
+    float top = -INFINITY;
+    for (int k = lane; k < p.splits; k += 32) top = fmaxf(top, a.part_ml[(at + (long long)k * C::MQ) * 2]);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    if (top == -INFINITY) top = 0.f;
+    constexpr int PER = DHP / 32;
+    float acc[PER], l = 0.f;
+#pragma unroll
+    for (int d = 0; d < PER; ++d) acc[d] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < p.splits; ++k) {
+      const long long pr = at + (long long)k * C::MQ;
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + pr * 2);
+      const float f = ex2_approx(ml.x - top);
+      l = fmaf(ml.y, f, l);
+#pragma unroll
+      for (int d = 0; d < PER; ++d) acc[d] = fmaf(a.part_o[pr * DHP + d * 32 + lane], f, acc[d]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const long long o = ((long long)(it.tok0 + i) * a.hq + it.h * a.group + gr - i * a.group) * a.dh;
+#pragma unroll
+    for (int d = 0; d < PER; ++d) {
+      const int dim = d * 32 + lane;
+      if (dim < a.dh) {
+        if (a.type == kElemF16) static_cast<__half*>(a.out)[o + dim] = __float2half_rn(acc[d] * inv);
+        else static_cast<__nv_bfloat16*>(a.out)[o + dim] = __float2bfloat16_rn(acc[d] * inv);
+      }
+    }
+  }
+}
+
+}  // namespace b200l

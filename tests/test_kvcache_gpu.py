@@ -315,6 +315,16 @@ def test_attention_long_and_short_together(pkg, cuda_ok, kind, dh, P):
         assert torch.equal(a, run_attention(pkg, s))
 
 
+@pytest.mark.parametrize("kind,dh,hq,hkv", [("int8", 32, 8, 4), ("fp8", 64, 4, 4), ("int8", 128, 12, 3), ("fp8", 256, 4, 4)])
+def test_attention_many_row_tiles(pkg, cuda_ok, kind, dh, hq, hkv):
+    """More row tiles than SMs, ragged, some requests idle, some with a single new token."""
+    rng = random.Random(dh)
+    new = [rng.choice([0, 0, 1, 60, 129, 200]) for _ in range(90)] + [300]
+    lens = [n + rng.choice([0, 0, 1, 37]) for n in new]
+    for causal in (True, False):
+        check_attention(pkg, attention_case(pkg, dh, kind, "fp16", hq, hkv, dh, 32, lens, new, causal))
+
+
 def test_attention_empty_rows(pkg, cuda_ok):
     """No keys at all; fewer keys than new tokens (the first rows see none); tokens past the plan's."""
     s = attention_case(pkg, 12, "int8", "fp16", 4, 2, 64, 16, [0, 3, 20], [2, 5, 4])
