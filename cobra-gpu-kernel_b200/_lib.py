@@ -54,6 +54,9 @@ ERRORS = {
 }
 
 
+ERR_WORKSPACE = -4
+
+
 class LayerDesc(ctypes.Structure):
     """Mirror of ``b200l_layer_desc``."""
 

@@ -17,15 +17,16 @@
 // cache; the codes themselves are then 0.
 //
 // A run is a stretch of tokens whose slots follow one another inside a page;
-// each page's new tokens have to be one run. A block takes the runs that begin
-// in its window of W tokens, for one head of K or V:
-//   1. max |x| of every token of those runs (lanes share a token, 8 dims each),
-//   2. a warp per run: the page's scale, and the older codes if it grew,
-//   3. codes of every token.
-// The second look at x comes from L1/L2: a window is W tokens of one head.
+// each page's new tokens have to be one run. A warp takes the runs that begin
+// in its window of W tokens, for one head of K or V, one after another: lanes
+// share a token (8 dims each) and hold up to 8 tokens each of 16-bit input, all
+// in flight together; then the
+// page's scale, the older codes if it grew, and the new codes. Nothing is
+// shared between warps. A longer run is looked at twice, the second time from
+// L1 / L2.
 //
 // Bound: HBM, 2 (or 4) bytes read and 1 written per value; a decode step is a
-// few microseconds of latency, so W shrinks to a token per warp there.
+// few microseconds of latency, so W shrinks to a token there.
 #pragma once
 
 #include "kv_common.cuh"
@@ -39,11 +40,8 @@ struct KvAppendArgs {
   int vec[2];                    // rows are read in 16-byte pieces
   const long long* slots;
   long long tokens, num_slots;
-  int type, dh, window;
+  int type, dh, window, windows;
 };
-
-constexpr int kKvAppendThreads = 256;
-constexpr int kKvAppendMaxTokens = 64 + 128;   // window + the longest run
 
 template <int KIND>
 __device__ __forceinline__ float kv_scale_for(float amax) {
@@ -58,16 +56,35 @@ __device__ __forceinline__ float kv_scale_for(float amax) {
   }
 }
 
-// Code of x at scale s; s == 0 only where every x is 0.
+// Code of x / s, correctly rounded as a quotient first. The quotient by way of
+// the reciprocal is off by less than 2^-22 of at most 127: where that could
+// matter, within 2^-13 of a tie, it is divided.
+__device__ __forceinline__ uint32_t kv_code_int8(float x, float s, float inv) {
+  float r = x * inv;
+  if (fabsf(r - rintf(r)) > 0.49987f) r = __fdiv_rn(x, s);
+  const int c = __float2int_rn(r);
+  return (uint32_t)max(-127, min(127, c)) & 0xffu;
+}
+// Four values at scale s. A scale of 0 (all of them 0) or not-a-number gives 0;
+// a power of two divides exactly by its reciprocal.
 template <int KIND>
-__device__ __forceinline__ uint32_t kv_code(float x, float s, float inv) {
+__device__ __forceinline__ uint32_t kv_code4(float a, float b, float c, float d, float s, float inv) {
+  if (!(s > 0.f)) return 0;
   if constexpr (KIND == kKvInt8) {
-    if (!(s > 0.f)) return 0;
-    const int c = __float2int_rn(__fdiv_rn(x, s));
-    return (uint32_t)max(-127, min(127, c)) & 0xffu;
+    // (the reciprocal of a scale near the ends of the range is no use)
+    if (!(s > 1e-30f && s < 1e30f)) {
+      const float q[4] = {__fdiv_rn(a, s), __fdiv_rn(b, s), __fdiv_rn(c, s), __fdiv_rn(d, s)};
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= ((uint32_t)max(-127, min(127, __float2int_rn(q[i]))) & 0xffu) << (8 * i);
+      return w;
+    }
+    return kv_code_int8(a, s, inv) | kv_code_int8(b, s, inv) << 8 | kv_code_int8(c, s, inv) << 16 |
+           kv_code_int8(d, s, inv) << 24;
   } else {
-    if (!(s > 0.f)) return 0;
-    return __nv_cvt_float_to_fp8(x * inv, __NV_SATFINITE, __NV_E4M3);   // s is a power of two: exact
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
   }
 }
 
@@ -78,141 +95,166 @@ __device__ __forceinline__ float kv_value(uint32_t c) {
   return __half2float(__half(h));
 }
 
-// Eight dims [d0, d0 + 8) of one token and head as fp32, zero past dh.
-__device__ __forceinline__ void kv_load8(const void* x, long long base, long long sd, int d0, int dh, int type, int vec,
-                                         float (&f)[8]) {
-  if (vec && d0 + 8 <= dh) {
-    if (type == kElemF32) {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + base + d0);
-      const float4 a = p[0], b = p[1];
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __half*>(x) + base + d0);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight dims of one token and head as they come: 16 bytes of a 16-bit type, 32
+// of fp32; zero past dh.
+template <int ESZ>
+struct KvPiece {
+  uint32_t w[ESZ * 2];
+  __device__ __forceinline__ void load(const void* x, long long base, long long sd, int d0, int dh, int vec) {
+    if (vec && d0 + 8 <= dh) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + (base + d0) * ESZ);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 p;
-        if (type == kElemF16) p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        else p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-        f[2 * i] = p.x;
-        f[2 * i + 1] = p.y;
+      for (int i = 0; i < ESZ / 2; ++i) {
+        const uint4 u = p[i];
+        w[4 * i] = u.x;
+        w[4 * i + 1] = u.y;
+        w[4 * i + 2] = u.z;
+        w[4 * i + 3] = u.w;
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = d0 + i < dh;
+      const long long at = base + (d0 + i) * sd;
+      if constexpr (ESZ == 4) {
+        w[i] = in ? static_cast<const uint32_t*>(x)[at] : 0u;
+      } else {
+        const uint32_t h = in ? static_cast<const unsigned short*>(x)[at] : 0u;
+        if (i & 1) w[i / 2] |= h << 16;
+        else w[i / 2] = h;
       }
     }
-    return;
   }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = d0 + i < dh ? load_elem(x, base + (d0 + i) * sd, type) : 0.f;
-}
+    for (int i = 0; i < ESZ * 2; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ float2 two(int i, int type) const {   // dims 2i, 2i + 1
+    if constexpr (ESZ == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if (type == kElemF16) return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+  }
+  // max(m, |x|), not-a-number if any is
+  __device__ __forceinline__ float amax(float m, int type) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = two(i, type);
+      m = (fabsf(f.x) <= m || m != m) ? m : fabsf(f.x);
+      m = (fabsf(f.y) <= m || m != m) ? m : fabsf(f.y);
+    }
+    return m;
+  }
+  template <int KIND>
+  __device__ __forceinline__ uint2 codes(float s, float inv, int type) const {
+    const float2 a = two(0, type), b = two(1, type), c = two(2, type), d = two(3, type);
+    return make_uint2(kv_code4<KIND>(a.x, a.y, b.x, b.y, s, inv), kv_code4<KIND>(c.x, c.y, d.x, d.y, s, inv));
+  }
+};
 
-template <int DHP, int KIND>
-__global__ void __launch_bounds__(kKvAppendThreads) kv_append_kernel(KvAppendArgs a) {
+template <int DHP, int KIND, int ESZ>
+__global__ void __launch_bounds__(256, 2) kv_append_kernel(KvAppendArgs a) {
   pdl_wait_then_release();
   constexpr int LPT = DHP / 8;                    // lanes that share a token
   constexpr int TPW = 32 / LPT;                   // tokens of a warp at a time
-  constexpr int NW = kKvAppendThreads / 32;
-  __shared__ long long s_slot[kKvAppendMaxTokens];
-  __shared__ float s_val[kKvAppendMaxTokens];     // max |x|, then the scale of the token's run
-  __shared__ unsigned char s_lead[kKvAppendMaxTokens];
-  __shared__ int s_end;                           // tokens from the window's start to its last run's end
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int P = a.c.page, head = blockIdx.y, which = blockIdx.z;
-  const long long t0 = (long long)blockIdx.x * a.window;
+  constexpr int U = 16 / ESZ;                     // ... and how many times at once
+  const int lane = threadIdx.x & 31;
+  const unsigned id = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int win = (int)(id / (2u * a.c.heads));
+  const int hk = (int)(id - win * (2u * a.c.heads));   // neighbours share tokens: their rows lie side by side
+  if (win >= a.windows) return;
+  const int head = hk >> 1, which = hk & 1, P = a.c.page;
+  const long long t0 = (long long)win * a.window;
   const int W = (int)min((long long)a.window, a.tokens - t0);
-  const int reach = (int)min((long long)W + P - 1, a.tokens - t0);
   uint8_t* codes = which ? a.c.v : a.c.k;
   float* scales = which ? a.c.v_scale : a.c.k_scale;
   const void* x = a.x[which];
   const long long st = a.st[which], sd = a.sd[which], xh = head * a.sh[which];
+  const int sub = lane / LPT, d0 = (lane % LPT) * 8, vec = a.vec[which];
 
-  // Slots of the window and of the tokens that its last run may reach; whether
-  // a token leads a run, or goes on the one before it (2: in no run).
-  if (tid == 0) s_end = reach;
-  for (int i = tid; i < reach; i += kKvAppendThreads) {
-    const long long s = a.slots[t0 + i];
-    const long long before = t0 + i > 0 ? a.slots[t0 + i - 1] : -1;
-    const bool in = s >= 0 && s < a.num_slots;
-    s_slot[i] = s;
-    s_lead[i] = !in ? 2 : (before < 0 || s != before + 1 || (s & (P - 1)) == 0) ? 1 : 0;
+  // Whether token t leads a run (1), goes on the one before it (0), or has no slot (2).
+  auto kind_of = [&](long long t) {
+    const long long s = a.slots[t], before = t > 0 ? a.slots[t - 1] : -1;
+    if (s < 0 || s >= a.num_slots) return 2;
+    return before < 0 || s != before + 1 || (s & (P - 1)) == 0 ? 1 : 0;
+  };
+  unsigned long long lead = 0, stop = 0;          // tokens of the window that lead; that do not go on
+  for (int i = 0; i < W; i += 32) {
+    const int k = i + lane < W ? kind_of(t0 + i + lane) : 2;
+    lead |= (unsigned long long)__ballot_sync(0xffffffffu, k == 1) << i;
+    stop |= (unsigned long long)__ballot_sync(0xffffffffu, k != 0 && i + lane < W) << i;
   }
-  __syncthreads();
-  // Tokens [begin, end): the runs led from inside the window.
-  int begin = 0;
-  while (begin < W && s_lead[begin] != 1) ++begin;
-  if (begin == W) return;
-  // The last of them may go on past the window, to the first token that does not.
-  for (int i = W + tid; i < reach; i += kKvAppendThreads)
-    if (s_lead[i] != 0) atomicMin(&s_end, i);
-  __syncthreads();
-  const int end = s_end;
-
-  const int sub = lane / LPT, d0 = (lane % LPT) * 8;
-  for (int i0 = begin + warp * TPW; i0 < end; i0 += NW * TPW) {
-    const int i = i0 + sub;
-    float m = 0.f;
-    if (i < end && s_lead[i] != 2) {
-      float f[8];
-      kv_load8(x, (t0 + i) * st + xh, sd, d0, a.dh, a.type, a.vec[which], f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) m = (fabsf(f[k]) <= m || m != m) ? m : fabsf(f[k]);   // not-a-number stays
+  while (lead) {
+    const int i = __ffsll((long long)lead) - 1;
+    lead &= lead - 1;
+    const unsigned long long after = i < 63 ? stop & (~0ull << (i + 1)) : 0;
+    int len;
+    if (after) {
+      len = __ffsll((long long)after) - 1 - i;
+    } else {                                      // on past the window
+      len = W - i;
+      for (long long t = t0 + W; t < a.tokens; t += 32) {
+        const unsigned m = __ballot_sync(0xffffffffu, t + lane >= a.tokens || kind_of(t + lane) != 0);
+        const int n = m ? __ffs(m) - 1 : 32;
+        len += n;
+        if (n < 32) break;
+      }
     }
-#pragma unroll
-    for (int o = LPT / 2; o > 0; o >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, m, o);
-      m = (y <= m || m != m) ? m : y;
-    }
-    if (i < end && d0 == 0) s_val[i] = m;
-  }
-  __syncthreads();
+    const long long slot = a.slots[t0 + i];
+    const long long page = slot >> a.c.log2_page;
+    const int place = (int)(slot & (P - 1));
+    float* sp = scales + page * a.c.heads + head;
+    const float was = place ? *sp : 0.f;
+    const long long row0 = (page * a.c.heads + head) << a.c.log2_page;
 
-  for (int i = begin + warp; i < end; i += NW) {
-    if (s_lead[i] != 1) continue;                 // (warp-uniform)
-    int len = 1;
-    while (i + len < end && s_lead[i + len] == 0) ++len;
+    KvPiece<ESZ> f[U];
+    const long long at0 = (t0 + i + sub) * st + xh, at1 = TPW * st;
+    auto load = [&](int from) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = from + u * TPW;
+        if (j >= len) break;                      // (warp-uniform)
+        if (j + sub < len) f[u].load(x, at0 + (j / TPW) * at1, sd, d0, a.dh, vec);
+        else f[u].zero();
+      }
+    };
     float m = 0.f;
-    for (int j = lane; j < len; j += 32) {
-      const float y = s_val[i + j];
-      m = (y <= m || m != m) ? m : y;
+    for (int from = 0; from < len; from += U * TPW) {
+      load(from);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (from + u * TPW >= len) break;
+        m = f[u].amax(m, a.type);
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float y = __shfl_xor_sync(0xffffffffu, m, o);
       m = (y <= m || m != m) ? m : y;
     }
-    const long long page = s_slot[i] >> a.c.log2_page;
-    const int place = (int)(s_slot[i] & (P - 1));
-    float* sp = scales + page * a.c.heads + head;
-    const float was = place ? *sp : 0.f;
     const float want = kv_scale_for<KIND>(m);
     const float now = (want <= was || was != was) ? was : want;   // not-a-number stays
     __syncwarp();
     if (lane == 0) *sp = now;
-    for (int j = lane; j < len; j += 32) s_val[i + j] = now;
     if (place && now > was) {                     // the older codes move to the new scale
-      const float f = __fdiv_rn(was, now);
-      uint32_t* row = reinterpret_cast<uint32_t*>(codes + ((page * a.c.heads + head) << a.c.log2_page) * DHP);
+      const float r = __fdiv_rn(was, now);
+      uint32_t* row = reinterpret_cast<uint32_t*>(codes + row0 * DHP);
       for (int j = lane; j < place * DHP / 4; j += 32) {
         const uint32_t w = row[j];
-        uint32_t o = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o |= kv_code<KIND>(kv_value<KIND>((w >> (8 * k)) & 0xffu) * f, 1.f, 1.f) << (8 * k);
-        row[j] = o;
+        row[j] = kv_code4<KIND>(kv_value<KIND>(w & 0xffu) * r, kv_value<KIND>((w >> 8) & 0xffu) * r,
+                                kv_value<KIND>((w >> 16) & 0xffu) * r, kv_value<KIND>(w >> 24) * r, 1.f, 1.f);
       }
     }
-  }
-  __syncthreads();
-
-  for (int i = begin + warp * TPW + sub; i < end; i += NW * TPW) {
-    if (s_lead[i] == 2) continue;
-    float f[8];
-    kv_load8(x, (t0 + i) * st + xh, sd, d0, a.dh, a.type, a.vec[which], f);
-    const float s = s_val[i], inv = KIND == kKvE4M3 ? __fdiv_rn(1.0f, s) : 0.f;
-    uint32_t w[2] = {0, 0};
+    const float inv = __fdiv_rn(1.0f, now);
+    for (int from = 0; from < len; from += U * TPW) {
+      if (len > U * TPW) load(from);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k >> 2] |= kv_code<KIND>(f[k], s, inv) << (8 * (k & 3));
-    const long long slot = s_slot[i];
-    const long long row = (((slot >> a.c.log2_page) * a.c.heads + head) << a.c.log2_page) + (slot & (P - 1));
-    *reinterpret_cast<uint2*>(codes + row * DHP + d0) = make_uint2(w[0], w[1]);
+      for (int u = 0; u < U; ++u) {
+        const int j = from + u * TPW + sub;
+        if (j - sub >= len) break;
+        if (j < len) *reinterpret_cast<uint2*>(codes + (row0 + place + j) * DHP + d0) = f[u].template codes<KIND>(now, inv, a.type);
+      }
+    }
   }
 }
 
@@ -225,47 +267,66 @@ struct KvReadArgs {
 };
 
 // Value = code * scale, rounded once; slots outside the cache read as 0.
-// A lane takes 8 codes of a token and head, K and V alike. Bound: HBM.
+// A lane takes 8 codes of a token and head, K and V alike, two pieces at a time.
+// Bound: HBM.
 template <int DHP, int KIND>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvReadArgs a) {
   pdl_wait_then_release();
   constexpr int LPT = DHP / 8;
-  const long long items = a.n * a.c.heads * LPT;
   const bool vec = a.dh % 8 == 0;
-  for (long long it = (long long)blockIdx.x * 256 + threadIdx.x; it < items; it += (long long)gridDim.x * 256) {
-    const int d0 = (int)(it % LPT) * 8;
-    const long long th = it / LPT;
-    const int head = (int)(th % a.c.heads);
-    if (d0 >= a.dh) continue;
-    const long long slot = a.slots[th / a.c.heads];
-    const bool in = slot >= 0 && slot < a.num_slots;
-    const long long ph = in ? (slot >> a.c.log2_page) * a.c.heads + head : 0;
-    const long long row = (ph << a.c.log2_page) + (in ? slot & (a.c.page - 1) : 0);
+  // Lanes of a token and head; (token, head) pairs by 32-bit division.
+  const long long pairs = a.n * a.c.heads, step = (long long)gridDim.x * 256 / LPT;
+  const int d0 = (threadIdx.x % LPT) * 8;
+  if (d0 >= a.dh) return;
+  for (long long th0 = ((long long)blockIdx.x * 256 + threadIdx.x) / LPT; th0 < pairs; th0 += 2 * step) {
+    uint2 w[2][2];
+    float s[2][2];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const uint2 w = in ? *reinterpret_cast<const uint2*>((which ? a.c.v : a.c.k) + row * DHP + d0) : make_uint2(0, 0);
-      const float s = in ? (which ? a.c.v_scale : a.c.k_scale)[ph] : 0.f;
-      float f[8];
+    for (int u = 0; u < 2; ++u) {
+      const long long th = th0 + u * step;
+      w[u][0] = w[u][1] = make_uint2(0, 0);
+      s[u][0] = s[u][1] = 0.f;
+      if (th >= pairs) continue;
+      const long long tok = pairs <= 0xffffffffLL ? (long long)((unsigned)th / (unsigned)a.c.heads) : th / a.c.heads;
+      const int head = (int)(th - tok * a.c.heads);
+      const long long slot = a.slots[tok];
+      if (slot < 0 || slot >= a.num_slots) continue;
+      const long long ph = (slot >> a.c.log2_page) * a.c.heads + head;
+      const long long at = ((ph << a.c.log2_page) + (slot & (a.c.page - 1))) * DHP + d0;
+      w[u][0] = *reinterpret_cast<const uint2*>(a.c.k + at);
+      w[u][1] = *reinterpret_cast<const uint2*>(a.c.v + at);
+      s[u][0] = a.c.k_scale[ph];
+      s[u][1] = a.c.v_scale[ph];
+    }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = kv_value<KIND>(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 0xffu) * s;
-      const long long o = th * a.dh + d0;
-      if (vec) {
-        if (a.type == kElemF32) {
-          float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out[which]) + o);
-          p[0] = make_float4(f[0], f[1], f[2], f[3]);
-          p[1] = make_float4(f[4], f[5], f[6], f[7]);
+    for (int u = 0; u < 2; ++u) {
+      const long long th = th0 + u * step;
+      if (th >= pairs) break;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          f[k] = kv_value<KIND>(((k < 4 ? w[u][which].x : w[u][which].y) >> (8 * (k & 3))) & 0xffu) * s[u][which];
+        const long long o = th * a.dh + d0;
+        if (vec) {
+          if (a.type == kElemF32) {
+            float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out[which]) + o);
+            p[0] = make_float4(f[0], f[1], f[2], f[3]);
+            p[1] = make_float4(f[4], f[5], f[6], f[7]);
+          } else {
+            *reinterpret_cast<uint4*>(static_cast<__half*>(a.out[which]) + o) =
+                make_uint4(pack_elem2(f[0], f[1], a.type), pack_elem2(f[2], f[3], a.type),
+                           pack_elem2(f[4], f[5], a.type), pack_elem2(f[6], f[7], a.type));
+          }
         } else {
-          *reinterpret_cast<uint4*>(static_cast<__half*>(a.out[which]) + o) =
-              make_uint4(pack_elem2(f[0], f[1], a.type), pack_elem2(f[2], f[3], a.type),
-                         pack_elem2(f[4], f[5], a.type), pack_elem2(f[6], f[7], a.type));
-        }
-      } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (d0 + k >= a.dh) break;
-          if (a.type == kElemF32) static_cast<float*>(a.out[which])[o + k] = f[k];
-          else if (a.type == kElemF16) static_cast<__half*>(a.out[which])[o + k] = __float2half_rn(f[k]);
-          else static_cast<__nv_bfloat16*>(a.out[which])[o + k] = __float2bfloat16_rn(f[k]);
+          for (int k = 0; k < 8; ++k) {
+            if (d0 + k >= a.dh) break;
+            if (a.type == kElemF32) static_cast<float*>(a.out[which])[o + k] = f[k];
+            else if (a.type == kElemF16) static_cast<__half*>(a.out[which])[o + k] = __float2half_rn(f[k]);
+            else static_cast<__nv_bfloat16*>(a.out[which])[o + k] = __float2bfloat16_rn(f[k]);
+          }
         }
       }
     }

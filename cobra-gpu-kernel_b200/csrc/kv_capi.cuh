@@ -97,17 +97,19 @@ int kv_plan_run(const b200l_kv_plan_desc* d, cudaStream_t st) {
 // ---------------------------------------------------------------- append, read
 template <int DHP, int KIND>
 int kv_append_t(const KvAppendArgs& a, cudaStream_t st) {
-  const long long blocks = (a.tokens + a.window - 1) / a.window;
-  cudaError_t e = launch_pdl(kv_append_kernel<DHP, KIND>, dim3((unsigned)blocks, (unsigned)a.c.heads, 2),
-                             dim3(kKvAppendThreads), 0, st, a);
+  const long long blocks = ((long long)a.windows * a.c.heads * 2 + 7) / 8;
+  if (blocks > 0x0fffffffLL) return fail(B200L_ERR_BAD_SHAPE, "kv_append: too many tokens and heads");
+  cudaError_t e = a.type == B200L_DTYPE_F32
+                      ? launch_pdl(kv_append_kernel<DHP, KIND, 4>, dim3((unsigned)blocks), dim3(256), 0, st, a)
+                      : launch_pdl(kv_append_kernel<DHP, KIND, 2>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   if (e != cudaSuccess) return cuda_fail(e, "kv_append_kernel");
   return check_launch("kv_append_kernel");
 }
 
 template <int DHP, int KIND>
 int kv_read_t(const KvReadArgs& a, int sms, cudaStream_t st) {
-  const long long blocks = (a.n * a.c.heads * (DHP / 8) + 255) / 256;
-  const long long most = 16ll * sms;
+  const long long blocks = (a.n * a.c.heads * (DHP / 8) + 511) / 512;   // two pieces a lane
+  const long long most = 32ll * sms;
   cudaError_t e = launch_pdl(kv_read_kernel<DHP, KIND>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, a);
   if (e != cudaSuccess) return cuda_fail(e, "kv_read_kernel");
   return check_launch("kv_read_kernel");
@@ -154,9 +156,10 @@ int kv_append_run(const b200l_kv_cache* cache, const b200l_kv_rows* rows, const 
   a.num_slots = cache->num_pages * cache->page_size;
   a.type = rows->dtype;
   a.dh = cache->head_dim;
-  // A window of 64 tokens a block where that fills the GPU twice over; else one
-  // token for each of the block's token groups, for latency.
-  a.window = tokens * cache->num_heads * 2 >= 64ll * 2 * dev.sms ? 64 : 8;
+  // Windows of up to 64 tokens a warp, while there are 32 warps for every SM.
+  a.window = 1;
+  while (a.window < 64 && tokens * cache->num_heads * 2 / (a.window * 2) >= 32ll * dev.sms) a.window *= 2;
+  a.windows = (int)((tokens + a.window - 1) / a.window);
 #define KV_CALL(D, K) kv_append_t<D, K>(a, st)
   KV_DISPATCH(cache->head_dim, cache->kind, KV_CALL)
 #undef KV_CALL
@@ -343,9 +346,9 @@ int kv_attention_run(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, v
   if (!d->q || !d->out || !d->block_table || !d->seq_lens || !d->cu_new || !d->cu_pages)
     return fail(B200L_ERR_NULL_POINTER, "kv_attention: NULL pointer");
   if (misaligned(d->q, 2) || misaligned(d->out, 4)) return fail(B200L_ERR_ALIGNMENT, "kv_attention: q or out is misaligned");
-  if (!ws) return fail(B200L_ERR_NULL_POINTER, "workspace is NULL");
   if (misaligned(ws, 1024)) return fail(B200L_ERR_ALIGNMENT, "workspace must be 1024-byte aligned");
-  if (ws_bytes < p.total) return fail(B200L_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", ws_bytes, p.total);
+  if (!ws || ws_bytes < p.total)
+    return fail(B200L_ERR_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", ws ? ws_bytes : 0, p.total);
   uint8_t* w = static_cast<uint8_t*>(ws);
   p.a.part_o = reinterpret_cast<float*>(w + p.off_o);
   p.a.part_ml = p.a.part_o + (size_t)p.pieces * p.M * p.dhp;

@@ -18,7 +18,7 @@ current stream of their tensors' device through the sm_100a library
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
@@ -73,10 +73,12 @@ def new_kv_cache(num_pages: int, num_heads: int, head_dim: int, *, page_size: in
 
 
 # ---------------------------------------------------------------- checks
-def _on(device: torch.device, **tensors: torch.Tensor) -> None:
+# Each operator asks once whether everything fits (a decode step's calls are
+# short); where something does not, the functions here say what.
+def _on(index: int, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
 
 
 def _ints(dtype: torch.dtype, **tensors: torch.Tensor) -> None:
@@ -87,41 +89,62 @@ def _ints(dtype: torch.dtype, **tensors: torch.Tensor) -> None:
             raise ValueError(f"{name} must be contiguous")
 
 
+def _cuda(t: torch.Tensor, name: str) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise RuntimeError(f"{name} is on {t.device}: the cache runs only on CUDA (sm_100a) devices; there is no CPU path")
+    return index
+
+
 def _table_stride(table: torch.Tensor, requests: int) -> int:
     if table.dtype != torch.int32:
         raise TypeError(f"block_table must be torch.int32, got {table.dtype}")
     if table.dim() != 2 or table.shape[0] != requests or table.shape[1] == 0:
         raise ValueError(f"block_table must be [{requests}, width], got {tuple(table.shape)}")
     width = table.shape[1]
-    if (width > 1 and table.stride(1) != 1) or (requests > 1 and table.stride(0) < width):
+    stride, inner = table.stride()
+    if (width > 1 and inner != 1) or (requests > 1 and stride < width):
         raise ValueError("block_table's rows must be contiguous and apart")
-    return table.stride(0) if requests > 1 else width
+    return stride if requests > 1 else width
 
 
-def _cuda(t: torch.Tensor, name: str) -> torch.device:
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} is on {t.device}: the cache runs only on CUDA (sm_100a) devices; there is no CPU path")
-    return t.device
-
-
-def _cache_desc(cache: KVCache, head_dim: int, device: torch.device) -> _lib.KVCacheDesc:
+def _refuse_cache(cache: KVCache, head_dim: int, index: int) -> None:
     k, v, ks, vs = cache
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2]:
         raise ValueError(f"cache shapes do not fit: codes {tuple(shape)}, {tuple(v.shape)}, "
                          f"scales {tuple(ks.shape)}, {tuple(vs.shape)}")
-    kind = _KINDS.get(k.dtype)
-    if kind is None or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+    if k.dtype not in _KINDS or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise TypeError(f"cache codes must be int8 or float8_e4m3fn and scales float32, got {k.dtype}, {v.dtype}, "
                         f"{ks.dtype}, {vs.dtype}")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache tensors must be contiguous")
-    if k.device != device or v.device != device or ks.device != device or vs.device != device:
-        raise ValueError(f"cache tensors must be on {device}")
-    if shape[3] != padded_head_dim(head_dim):
-        raise ValueError(f"cache rows have {shape[3]} columns, head_dim {head_dim} needs {padded_head_dim(head_dim)}")
-    return _lib.KVCacheDesc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), shape[0], shape[1], shape[2],
-                            head_dim, kind)
+    if any(t.get_device() != index for t in cache):
+        raise ValueError(f"cache tensors must be on cuda:{index}")
+    raise ValueError(f"cache rows have {shape[3]} columns, head_dim {head_dim} needs {padded_head_dim(head_dim)}")
+
+
+# Descriptors as the library reads them (the layouts of ``_lib.KVCacheDesc``,
+# ``KVPlanDesc``, ``KVRows`` and ``KVAttnDesc``), packed in one step.
+_pack_cache = struct.Struct("@PPPPqiiii").pack
+_pack_plan = struct.Struct("@PPPqPPPPPPPiiiii4x").pack
+_pack_rows = struct.Struct("@PPqqqqqqi4x").pack
+_pack_attn = struct.Struct("@PPqqPqPPPiiiiiiif").pack
+
+
+def _cache_desc(cache: KVCache, head_dim: int, index: int) -> bytes:
+    k, v, ks, vs = cache
+    shape = k.shape
+    kind = _KINDS.get(k.dtype)
+    scales = shape[:2]
+    f32 = torch.float32
+    if (kind is None or len(shape) != 4 or v.shape != shape or ks.shape != scales or vs.shape != scales or v.dtype != k.dtype
+            or ks.dtype != f32 or vs.dtype != f32 or not k.is_contiguous() or not v.is_contiguous()
+            or not ks.is_contiguous() or not vs.is_contiguous() or k.get_device() != index or v.get_device() != index
+            or ks.get_device() != index or vs.get_device() != index or shape[3] != padded_head_dim(head_dim)):
+        _refuse_cache(cache, head_dim, index)
+    pages, heads, page, _ = shape
+    return _pack_cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, page, head_dim, kind)
 
 
 # ---------------------------------------------------------------- workspaces
@@ -133,23 +156,24 @@ class _Workspace:
     def __init__(self) -> None:
         self._held: Dict[Tuple[int, int], list] = {}
 
-    def get(self, device: torch.device, stream: int, need: int) -> Tuple[int, int]:
-        key = (device.index, stream)
-        held = self._held.get(key)
-        if held is None:
-            held = self._held[key] = []
-        if not held or held[-1][2] < need:
-            size = max(need, 2 * held[-1][2] if held else 0)
-            buf = torch.empty(size + 1024, dtype=torch.uint8, device=device)
-            ptr = (buf.data_ptr() + 1023) // 1024 * 1024
-            _lib.check(_lib.lib().b200l_clear_status(ptr, stream))
-            held.append((buf, ptr, size))
-        return held[-1][1], held[-1][2]
+    def get(self, index: int, stream: int) -> Tuple[int, int]:
+        """(address, bytes), 0 bytes if there is none yet."""
+        held = self._held.get((index, stream))
+        return held[-1][:2] if held else (0, 0)
+
+    def grow(self, index: int, stream: int, need: int) -> Tuple[int, int]:
+        held = self._held.setdefault((index, stream), [])
+        size = max(need, 2 * held[-1][1] if held else 0)
+        buf = torch.empty(size + 1024, dtype=torch.uint8, device=torch.device("cuda", index))
+        ptr = (buf.data_ptr() + 1023) // 1024 * 1024
+        _lib.check(_lib.lib().b200l_clear_status(ptr, stream))
+        held.append((ptr, size, buf))
+        return ptr, size
 
     def check(self) -> None:
         for (index, stream), held in self._held.items():
             with torch.cuda.device(index):
-                for _, ptr, _ in held:
+                for ptr, _, _ in held:
                     _lib.check(_lib.lib().b200l_read_status(ptr, stream))
 
 
@@ -162,24 +186,12 @@ def kv_check_status() -> None:
     _workspace.check()
 
 
-class _Current:
-    """The device as the current one, and its current stream's handle."""
-
-    __slots__ = ("device", "other")
-
-    def __init__(self, device: torch.device) -> None:
-        self.device = device
-        self.other = None
-
-    def __enter__(self) -> int:
-        if torch.cuda.current_device() != self.device.index:
-            self.other = torch.cuda.device(self.device)
-            self.other.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.other is not None:
-            self.other.__exit__(*exc)
+def _on_device(call, index: int, *args):
+    """call(stream, *args) with device ``index`` current and its current stream."""
+    if torch.cuda.current_device() == index:
+        return call(torch._C._cuda_getCurrentRawStream(index), *args)
+    with torch.cuda.device(index):
+        return call(torch._C._cuda_getCurrentRawStream(index), *args)
 
 
 # ---------------------------------------------------------------- operators
@@ -197,32 +209,44 @@ def kv_plan(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.T
     their table entries and slots are -1: plan again with other ``new_lens``.
     ``max_tokens`` bounds the new tokens; entries past them are -1.
     """
-    dev = _cuda(old_lens, "old_lens")
-    _on(dev, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_count=free_count)
-    _ints(torch.int32, old_lens=old_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count)
-    if old_lens.dim() != 1 or new_lens.shape != old_lens.shape or old_lens.numel() == 0:
-        raise ValueError(f"old_lens and new_lens must be [requests], got {tuple(old_lens.shape)}, {tuple(new_lens.shape)}")
+    index = _cuda(old_lens, "old_lens")
     R = old_lens.numel()
-    table_stride = _table_stride(block_table, R)
-    if free_pages.dim() != 1 or free_count.numel() != 1:
-        raise ValueError("free_pages must be one-dimensional and free_count a single number")
-    if page_size not in PAGE_SIZES:
-        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
-    if max_tokens < 0:
-        raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
-    with _Current(dev) as stream:
-        # One allocation: slots (8 bytes each) first, then the int32 outputs.
-        ints = 2 * max_tokens + max_tokens + 2 * (R + 1) + 2
-        buf = torch.empty(ints, dtype=torch.int32, device=dev)
-        slots = buf[:2 * max_tokens].view(torch.int64)
-        positions, cu_new, cu_pages, info = buf[2 * max_tokens:].split((max_tokens, R + 1, R + 1, 2))
-        desc = _lib.KVPlanDesc(
-            old_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-            table_stride,
-            free_pages.data_ptr(), free_count.data_ptr(), cu_new.data_ptr(), cu_pages.data_ptr(), positions.data_ptr(),
-            slots.data_ptr(), info.data_ptr(), R, block_table.shape[1], page_size, free_pages.numel(), max_tokens)
-        _lib.check(_lib.lib().b200l_kv_plan(ctypes.byref(desc), stream))
-    return KVPlan(cu_new, cu_pages, positions, slots, info)
+    i32 = torch.int32
+    if (old_lens.dtype != i32 or new_lens.dtype != i32 or free_pages.dtype != i32 or free_count.dtype != i32
+            or old_lens.dim() != 1 or new_lens.shape != old_lens.shape or R == 0 or free_pages.dim() != 1
+            or free_count.numel() != 1 or not old_lens.is_contiguous() or not new_lens.is_contiguous()
+            or not free_pages.is_contiguous() or page_size not in PAGE_SIZES or max_tokens < 0
+            or new_lens.get_device() != index or block_table.get_device() != index or free_pages.get_device() != index
+            or free_count.get_device() != index):
+        _on(index, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_count=free_count)
+        _ints(i32, old_lens=old_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count)
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+        if max_tokens < 0:
+            raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
+        if free_pages.dim() != 1 or free_count.numel() != 1:
+            raise ValueError("free_pages must be one-dimensional and free_count a single number")
+        raise ValueError(f"old_lens and new_lens must be [requests], got {tuple(old_lens.shape)}, {tuple(new_lens.shape)}")
+    stride = _table_stride(block_table, R)
+    return _on_device(_plan, index, old_lens, new_lens, block_table, stride, free_pages, free_count, page_size, max_tokens)
+
+
+def _plan(stream, old_lens, new_lens, table, stride, free_pages, free_count, page_size, max_tokens) -> KVPlan:
+    R, width = table.shape
+    # One allocation: slots (8 bytes each), then the int32 outputs.
+    buf = torch.empty(3 * max_tokens + 2 * R + 4, dtype=torch.int32, device=old_lens.device)
+    at = buf.data_ptr()
+    slots, positions, cu_new, cu_pages, info = buf.split_with_sizes((2 * max_tokens, max_tokens, R + 1, R + 1, 2))
+    p_pos = at + 8 * max_tokens
+    p_new = p_pos + 4 * max_tokens
+    p_pages = p_new + 4 * (R + 1)
+    rc = _lib.lib().b200l_kv_plan(
+        _pack_plan(old_lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(), stride, free_pages.data_ptr(),
+                   free_count.data_ptr(), p_new, p_pages, p_pos, at, p_pages + 4 * (R + 1), R, width, page_size,
+                   free_pages.numel(), max_tokens), stream)
+    if rc:
+        _lib.check(rc)
+    return KVPlan(cu_new, cu_pages, positions, slots.view(torch.int64), info)
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: KVCache) -> None:
@@ -235,23 +259,32 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: KVCa
     one page have to follow one another in ``slots``, as ``kv_plan`` makes them.
     Values that are not finite make their page's scale not-a-number.
     """
-    dev = _cuda(k, "k")
-    if k.dim() != 3 or v.shape != k.shape:
-        raise ValueError(f"k and v must be [tokens, heads, head_dim], got {tuple(k.shape)}, {tuple(v.shape)}")
+    index = _cuda(k, "k")
     dtype = _DTYPES.get(k.dtype)
-    if dtype is None or v.dtype != k.dtype:
-        raise TypeError(f"k and v must both be fp32, fp16 or bf16, got {k.dtype}, {v.dtype}")
-    T, H, dh = k.shape
-    _on(dev, v=v, slots=slots)
-    _ints(torch.int64, slots=slots)
-    if slots.dim() != 1 or slots.numel() < T:
-        raise ValueError(f"slots must be [at least {T}], got {tuple(slots.shape)}")
-    if cache.k.dim() == 4 and cache.k.shape[1] != H:
-        raise ValueError(f"k has {H} heads, the cache {cache.k.shape[1]}")
-    with _Current(dev) as stream:
-        c = _cache_desc(cache, dh, dev)
-        rows = _lib.KVRows(k.data_ptr(), v.data_ptr(), k.stride(), v.stride(), dtype)
-        _lib.check(_lib.lib().b200l_kv_append(ctypes.byref(c), ctypes.byref(rows), slots.data_ptr(), T, stream))
+    if (dtype is None or v.dtype != k.dtype or k.dim() != 3 or v.shape != k.shape or v.get_device() != index
+            or slots.get_device() != index or slots.dtype != torch.int64 or not slots.is_contiguous() or slots.dim() != 1
+            or slots.shape[0] < k.shape[0] or cache[0].dim() != 4 or cache[0].shape[1] != k.shape[1]):
+        if k.dim() != 3 or v.shape != k.shape:
+            raise ValueError(f"k and v must be [tokens, heads, head_dim], got {tuple(k.shape)}, {tuple(v.shape)}")
+        if dtype is None or v.dtype != k.dtype:
+            raise TypeError(f"k and v must both be fp32, fp16 or bf16, got {k.dtype}, {v.dtype}")
+        _on(index, v=v, slots=slots)
+        _ints(torch.int64, slots=slots)
+        if slots.dim() != 1 or slots.numel() < k.shape[0]:
+            raise ValueError(f"slots must be [at least {k.shape[0]}], got {tuple(slots.shape)}")
+        if cache.k.dim() != 4:
+            _refuse_cache(cache, k.shape[2], index)
+        raise ValueError(f"k has {k.shape[1]} heads, the cache {cache.k.shape[1]}")
+    T, _, dh = k.shape
+    c = _cache_desc(cache, dh, index)
+    rows = _pack_rows(k.data_ptr(), v.data_ptr(), *k.stride(), *v.stride(), dtype)
+    _on_device(_append, index, c, rows, slots.data_ptr(), T)
+
+
+def _append(stream, c, rows, slots, T) -> None:
+    rc = _lib.lib().b200l_kv_append(c, rows, slots, T, stream)
+    if rc:
+        _lib.check(rc)
 
 
 def kv_read(slots: torch.Tensor, cache: KVCache, head_dim: int, *,
@@ -259,21 +292,25 @@ def kv_read(slots: torch.Tensor, cache: KVCache, head_dim: int, *,
     """The keys and values that the codes of ``slots`` (int64 ``[n]``) stand for,
     ``[n, heads, head_dim]`` each, rounded once to ``dtype``; slots outside the
     cache read as 0."""
-    dev = _cuda(slots, "slots")
-    _ints(torch.int64, slots=slots)
-    if slots.dim() != 1:
-        raise ValueError(f"slots must be [n], got {tuple(slots.shape)}")
+    index = _cuda(slots, "slots")
     code = _DTYPES.get(dtype)
-    if code is None:
+    if code is None or slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        _ints(torch.int64, slots=slots)
+        if slots.dim() != 1:
+            raise ValueError(f"slots must be [n], got {tuple(slots.shape)}")
         raise TypeError(f"dtype must be fp32, fp16 or bf16, got {dtype}")
-    with _Current(dev) as stream:
-        c = _cache_desc(cache, head_dim, dev)
-        n = slots.numel()
-        k = torch.empty((n, cache.k.shape[1], head_dim), dtype=dtype, device=dev)
-        v = torch.empty_like(k)
-        if n:
-            _lib.check(_lib.lib().b200l_kv_read(ctypes.byref(c), slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
-                                                stream))
+    c = _cache_desc(cache, head_dim, index)
+    return _on_device(_read, index, c, slots, cache.k.shape[1], head_dim, dtype, code)
+
+
+def _read(stream, c, slots, heads, dh, dtype, code) -> Tuple[torch.Tensor, torch.Tensor]:
+    n = slots.shape[0]
+    k = torch.empty((n, heads, dh), dtype=dtype, device=slots.device)
+    v = torch.empty_like(k)
+    if n:
+        rc = _lib.lib().b200l_kv_read(c, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code, stream)
+        if rc:
+            _lib.check(rc)
     return k, v
 
 
@@ -291,40 +328,52 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq
     ``scale`` is head_dim ** -0.5 if not given. A row that sees no key is 0, and
     so are rows past the plan's tokens. Returns ``out``, contiguous, q's dtype.
     """
-    dev = _cuda(q, "q")
+    index = _cuda(q, "q")
     if q.dim() != 3:
         raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
     T, hq, dh = q.shape
-    if q.stride(2) != 1 and dh > 1:
-        raise ValueError("q's dims must be contiguous")
-    _on(dev, block_table=block_table, seq_lens=seq_lens, cu_new=plan.cu_new, cu_pages=plan.cu_pages)
-    _ints(torch.int32, seq_lens=seq_lens, cu_new=plan.cu_new, cu_pages=plan.cu_pages)
-    R = seq_lens.numel()
-    if seq_lens.dim() != 1 or plan.cu_new.numel() != R + 1 or plan.cu_pages.numel() != R + 1:
-        raise ValueError(f"seq_lens [requests] and the plan's sums [requests + 1] do not fit: {R}, "
-                         f"{plan.cu_new.numel()}, {plan.cu_pages.numel()}")
-    table_stride = _table_stride(block_table, R)
-    if max_new < 0:
-        raise ValueError(f"max_new must not be negative, got {max_new}")
+    st, sh, sd = q.stride()
+    cu_new, cu_pages = plan.cu_new, plan.cu_pages
+    i32 = torch.int32
+    dtype = q.dtype
+    R = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    if ((dtype != torch.float16 and dtype != torch.bfloat16) or (sd != 1 and dh > 1) or seq_lens.dtype != i32
+            or cu_new.dtype != i32 or cu_pages.dtype != i32 or not seq_lens.is_contiguous() or not cu_new.is_contiguous()
+            or not cu_pages.is_contiguous() or cu_new.numel() != R + 1 or cu_pages.numel() != R + 1 or max_new < 0
+            or block_table.get_device() != index or seq_lens.get_device() != index or cu_new.get_device() != index
+            or cu_pages.get_device() != index):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"q must be fp16 or bf16, got {dtype}")
+        if sd != 1 and dh > 1:
+            raise ValueError("q's dims must be contiguous")
+        _on(index, block_table=block_table, seq_lens=seq_lens, cu_new=cu_new, cu_pages=cu_pages)
+        _ints(i32, seq_lens=seq_lens, cu_new=cu_new, cu_pages=cu_pages)
+        if max_new < 0:
+            raise ValueError(f"max_new must not be negative, got {max_new}")
+        raise ValueError(f"seq_lens [requests] and the plan's sums [requests + 1] do not fit: {tuple(seq_lens.shape)}, "
+                         f"{cu_new.numel()}, {cu_pages.numel()}")
+    stride = _table_stride(block_table, R)
     if out is None:
-        out = torch.empty((T, hq, dh), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        out = torch.empty((T, hq, dh), dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype or out.get_device() != index or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     if T == 0:
         return out
-    L = _lib.lib()
-    with _Current(dev) as stream:
-        c = _cache_desc(cache, dh, dev)
-        desc = _lib.KVAttnDesc(
-            q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), block_table.data_ptr(),
-            table_stride, seq_lens.data_ptr(), plan.cu_new.data_ptr(),
-            plan.cu_pages.data_ptr(), R, block_table.shape[1], T, hq, max_new, 1 if causal else 0, _DTYPES[q.dtype],
-            dh ** -0.5 if scale is None else scale)
-        need = L.b200l_kv_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(desc))
-        if need == 0:
-            raise _lib.B200LError(-1, _lib.last_error())
-        ws, size = _workspace.get(dev, stream, need)
-        _lib.check(L.b200l_kv_attention(ctypes.byref(c), ctypes.byref(desc), ws, size, stream))
+    c = _cache_desc(cache, dh, index)
+    desc = _pack_attn(q.data_ptr(), out.data_ptr(), st, sh, block_table.data_ptr(), stride, seq_lens.data_ptr(),
+                      cu_new.data_ptr(), cu_pages.data_ptr(), R, block_table.shape[1], T, hq, max_new, 1 if causal else 0,
+                      _DTYPES[dtype], dh ** -0.5 if scale is None else scale)
+    _on_device(_attention, index, index, c, desc)
     return out
+
+
+def _attention(stream, index, c, desc) -> None:
+    L = _lib.lib()
+    ws, size = _workspace.get(index, stream)
+    rc = L.b200l_kv_attention(c, desc, ws, size, stream)
+    if rc == _lib.ERR_WORKSPACE:
+        need = L.b200l_kv_attention_workspace_bytes(c, desc)
+        ws, size = _workspace.grow(index, stream, need)
+        rc = L.b200l_kv_attention(c, desc, ws, size, stream)
+    if rc:
+        _lib.check(rc)

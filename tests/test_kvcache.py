@@ -31,6 +31,20 @@ def test_descriptor_layout_matches_header(pkg, tmp_path, struct, cls):
     assert out == [ctypes.sizeof(D)] + [getattr(D, n).offset for n in names]
 
 
+def test_packed_descriptors_have_the_structs_layout(pkg):
+    """What kvcache.py packs in one step reads back field by field through the ctypes mirrors."""
+    from importlib import import_module
+    m, L = import_module(pkg.__name__ + ".kvcache"), pkg._lib
+    for pack, cls in ((m._pack_cache, L.KVCacheDesc), (m._pack_plan, L.KVPlanDesc), (m._pack_rows, L.KVRows),
+                      (m._pack_attn, L.KVAttnDesc)):
+        n = sum(3 if t is ctypes.c_int64 * 3 else 1 for _, t in cls._fields_)
+        d = cls.from_buffer_copy(pack(*range(1, n + 1)))
+        got = []
+        for f, t in cls._fields_:
+            got += list(getattr(d, f)) if t is ctypes.c_int64 * 3 else [getattr(d, f)]
+        assert got == list(range(1, n + 1))
+
+
 def cache_desc(pkg, **kw):
     d = dict(k=1024, v=1024, k_scale=1024, v_scale=1024, num_pages=4, num_heads=2, page_size=16, head_dim=64, kind=0)
     return pkg._lib.KVCacheDesc(**{**d, **kw})
