@@ -17,16 +17,19 @@
 // cache; the codes themselves are then 0.
 //
 // A run is a stretch of tokens whose slots follow one another inside a page;
-// each page's new tokens have to be one run. A warp takes the runs that begin
-// in its window of W tokens, for one head of K or V, one after another: lanes
-// share a token (8 dims each) and hold up to 8 tokens each of 16-bit input, all
-// in flight together; then the
-// page's scale, the older codes if it grew, and the new codes. Nothing is
-// shared between warps. A longer run is looked at twice, the second time from
+// each page's new tokens have to be one run. A group of GW warps takes the runs
+// that begin in its window of W tokens, for one head of K or V. A few runs (a
+// prompt's pages) are shared by the whole group, one run after another; many (a
+// decode batch's tokens) go to a warp each. Lanes share a token (8 dims each)
+// and hold 4 tokens, all in flight together and loaded once where GW suffices
+// for 64 tokens (dhp <= 128). Then the page's scale, the older codes if it grew,
+// and the new codes. What does not fit is looked at twice, the second time from
 // L1 / L2.
 //
-// Bound: HBM, 2 (or 4) bytes read and 1 written per value; a decode step is a
-// few microseconds of latency, so W shrinks to a token there.
+// Bound: HBM, 2 (or 4) bytes read and 1 written per value. A run is a chain of
+// some 3000 clocks (slots, values and scale, maximum, codes), so about 45 KB of
+// values have to be on their way in an SM: 32 warps of 2 KB. A decode step is
+// that chain once.
 #pragma once
 
 #include "kv_common.cuh"
@@ -56,36 +59,47 @@ __device__ __forceinline__ float kv_scale_for(float amax) {
   }
 }
 
-// Code of x / s, correctly rounded as a quotient first. The quotient by way of
-// the reciprocal is off by less than 2^-22 of at most 127: where that could
-// matter, within 2^-13 of a tie, it is divided.
-__device__ __forceinline__ uint32_t kv_code_int8(float x, float s, float inv) {
-  float r = x * inv;
-  if (fabsf(r - rintf(r)) > 0.49987f) r = __fdiv_rn(x, s);
-  const int c = __float2int_rn(r);
-  return (uint32_t)max(-127, min(127, c)) & 0xffu;
-}
-// Four values at scale s. A scale of 0 (all of them 0) or not-a-number gives 0;
-// a power of two divides exactly by its reciprocal.
+// Codes of four values at scale s: the quotient as fp32 rounds it, rounded to the
+// code. A scale of 0 (all of them 0) or not-a-number gives 0; a power of two
+// divides exactly by its reciprocal.
 template <int KIND>
 __device__ __forceinline__ uint32_t kv_code4(float a, float b, float c, float d, float s, float inv) {
-  if (!(s > 0.f)) return 0;
   if constexpr (KIND == kKvInt8) {
-    // (the reciprocal of a scale near the ends of the range is no use)
-    if (!(s > 1e-30f && s < 1e30f)) {
-      const float q[4] = {__fdiv_rn(a, s), __fdiv_rn(b, s), __fdiv_rn(c, s), __fdiv_rn(d, s)};
-      uint32_t w = 0;
+    // The quotient by way of the reciprocal is off by less than 2^-22 of at most
+    // 127: where that could matter, within 2^-13 of a tie, it is divided. Adding
+    // 1.5 2^23 rounds to a whole number, ties to even, and leaves it in the low
+    // bits; it stays in [-127, 127] since s >= max|x| / 127 but for its rounding.
+    const float big = 12582912.0f;
+    float q[4] = {a * inv, b * inv, c * inv, d * inv}, r[4];
+    float off = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w |= ((uint32_t)max(-127, min(127, __float2int_rn(q[i]))) & 0xffu) << (8 * i);
-      return w;
+    for (int i = 0; i < 4; ++i) {
+      r[i] = q[i] + big;
+      off = fmaxf(off, fabsf(q[i] - (r[i] - big)));
     }
-    return kv_code_int8(a, s, inv) | kv_code_int8(b, s, inv) << 8 | kv_code_int8(c, s, inv) << 16 |
-           kv_code_int8(d, s, inv) << 24;
+    // (nor is the reciprocal of a scale near the ends of the range any use)
+    if (off > 0.49987f || !(s > 1e-30f && s < 1e30f)) {
+      if (!(s > 0.f)) return 0;
+      const float x[4] = {a, b, c, d};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = __fdiv_rn(x[i], s) + big;
+    }
+    const uint32_t lo = __byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
   } else {
+    if (!(s > 0.f)) return 0;
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
   }
+}
+
+// Maximum, not-a-number if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
 
 template <int KIND>
@@ -137,13 +151,21 @@ struct KvPiece {
   }
   // max(m, |x|), not-a-number if any is
   __device__ __forceinline__ float amax(float m, int type) const {
+    if constexpr (ESZ == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = two(i, type);
-      m = (fabsf(f.x) <= m || m != m) ? m : fabsf(f.x);
-      m = (fabsf(f.y) <= m || m != m) ? m : fabsf(f.y);
+      for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(__uint_as_float(w[i])));
+      return m;
+    } else if (type == kElemF16) {
+      const __half2* h = reinterpret_cast<const __half2*>(w);
+      const __half2 x = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+      const float2 f = __half22float2(x);
+      return max_nan(m, max_nan(f.x, f.y));
+    } else {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+      const __nv_bfloat162 x = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+      const float2 f = __bfloat1622float2(x);
+      return max_nan(m, max_nan(f.x, f.y));
     }
-    return m;
   }
   template <int KIND>
   __device__ __forceinline__ uint2 codes(float s, float inv, int type) const {
@@ -152,17 +174,23 @@ struct KvPiece {
   }
 };
 
+// Warps of a group: as many as hold 64 tokens in registers, at most a block.
+__host__ __device__ constexpr int kv_append_group(int dhp) { return dhp <= 32 ? 2 : dhp <= 64 ? 4 : 8; }
+
 template <int DHP, int KIND, int ESZ>
-__global__ void __launch_bounds__(256, 2) kv_append_kernel(KvAppendArgs a) {
+__global__ void __launch_bounds__(256, ESZ == 2 ? 4 : 3) kv_append_kernel(KvAppendArgs a) {
   pdl_wait_then_release();
   constexpr int LPT = DHP / 8;                    // lanes that share a token
   constexpr int TPW = 32 / LPT;                   // tokens of a warp at a time
-  constexpr int U = 16 / ESZ;                     // ... and how many times at once
+  constexpr int U = 4;                            // ... and how many times at once
+  constexpr int GW = kv_append_group(DHP);
   const int lane = threadIdx.x & 31;
-  const unsigned id = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5, gw = warp % GW;
+  __shared__ float s_max[2][8];
+  const unsigned id = blockIdx.x * (8 / GW) + warp / GW;
   const int win = (int)(id / (2u * a.c.heads));
-  const int hk = (int)(id - win * (2u * a.c.heads));   // neighbours share tokens: their rows lie side by side
   if (win >= a.windows) return;
+  const int hk = (int)(id - win * (2u * a.c.heads));   // neighbours share tokens: their rows lie side by side
   const int head = hk >> 1, which = hk & 1, P = a.c.page;
   const long long t0 = (long long)win * a.window;
   const int W = (int)min((long long)a.window, a.tokens - t0);
@@ -184,9 +212,12 @@ __global__ void __launch_bounds__(256, 2) kv_append_kernel(KvAppendArgs a) {
     lead |= (unsigned long long)__ballot_sync(0xffffffffu, k == 1) << i;
     stop |= (unsigned long long)__ballot_sync(0xffffffffu, k != 0 && i + lane < W) << i;
   }
-  while (lead) {
+  const bool share = __popcll(lead) <= (GW + 1) / 2;   // (group-uniform)
+  const int wv = share ? gw : 0, nw = share ? GW : 1;
+  for (int nth = 0; lead; ++nth) {
     const int i = __ffsll((long long)lead) - 1;
     lead &= lead - 1;
+    if (!share && nth % GW != gw) continue;
     const unsigned long long after = i < 63 ? stop & (~0ull << (i + 1)) : 0;
     int len;
     if (after) {
@@ -208,51 +239,57 @@ __global__ void __launch_bounds__(256, 2) kv_append_kernel(KvAppendArgs a) {
     const long long row0 = (page * a.c.heads + head) << a.c.log2_page;
 
     KvPiece<ESZ> f[U];
-    const long long at0 = (t0 + i + sub) * st + xh, at1 = TPW * st;
+    // Piece u of this warp, counted from token `from`: TPW tokens, nw warps apart.
+    const long long at0 = (t0 + i + wv * TPW + sub) * st + xh, at1 = (long long)nw * TPW * st;
+    const int first = wv * TPW, span = nw * TPW;
     auto load = [&](int from) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = from + u * TPW;
+        const int j = from + first + u * span;
         if (j >= len) break;                      // (warp-uniform)
-        if (j + sub < len) f[u].load(x, at0 + (j / TPW) * at1, sd, d0, a.dh, vec);
+        if (j + sub < len) f[u].load(x, at0 + (from / span + u) * at1, sd, d0, a.dh, vec);
         else f[u].zero();
       }
     };
     float m = 0.f;
-    for (int from = 0; from < len; from += U * TPW) {
+    for (int from = 0; from < len; from += U * span) {
       load(from);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (from + u * TPW >= len) break;
+        if (from + first + u * span >= len) break;
         m = f[u].amax(m, a.type);
       }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, m, o);
-      m = (y <= m || m != m) ? m : y;
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (share) {                                  // (two buffers: the next run's maxima cannot overtake this one's readers)
+      if (lane == 0) s_max[nth & 1][warp] = m;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / GW), "n"(GW * 32) : "memory");
+#pragma unroll
+      for (int w = 0; w < GW; ++w) m = max_nan(m, s_max[nth & 1][warp / GW * GW + w]);
     }
     const float want = kv_scale_for<KIND>(m);
     const float now = (want <= was || was != was) ? was : want;   // not-a-number stays
     __syncwarp();
-    if (lane == 0) *sp = now;
+    if (lane == 0 && wv == 0) *sp = now;          // (everybody has read it)
     if (place && now > was) {                     // the older codes move to the new scale
       const float r = __fdiv_rn(was, now);
       uint32_t* row = reinterpret_cast<uint32_t*>(codes + row0 * DHP);
-      for (int j = lane; j < place * DHP / 4; j += 32) {
+      for (int j = wv * 32 + lane; j < place * DHP / 4; j += nw * 32) {
         const uint32_t w = row[j];
         row[j] = kv_code4<KIND>(kv_value<KIND>(w & 0xffu) * r, kv_value<KIND>((w >> 8) & 0xffu) * r,
                                 kv_value<KIND>((w >> 16) & 0xffu) * r, kv_value<KIND>(w >> 24) * r, 1.f, 1.f);
       }
     }
     const float inv = __fdiv_rn(1.0f, now);
-    for (int from = 0; from < len; from += U * TPW) {
-      if (len > U * TPW) load(from);
+    for (int from = 0; from < len; from += U * span) {
+      if (len > U * span) load(from);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = from + u * TPW + sub;
-        if (j - sub >= len) break;
-        if (j < len) *reinterpret_cast<uint2*>(codes + (row0 + place + j) * DHP + d0) = f[u].template codes<KIND>(now, inv, a.type);
+        const int j = from + first + u * span;
+        if (j >= len) break;
+        if (j + sub < len)
+          *reinterpret_cast<uint2*>(codes + (row0 + place + j + sub) * DHP + d0) = f[u].template codes<KIND>(now, inv, a.type);
       }
     }
   }

@@ -97,8 +97,9 @@ int kv_plan_run(const b200l_kv_plan_desc* d, cudaStream_t st) {
 // ---------------------------------------------------------------- append, read
 template <int DHP, int KIND>
 int kv_append_t(const KvAppendArgs& a, cudaStream_t st) {
-  const long long blocks = ((long long)a.windows * a.c.heads * 2 + 7) / 8;
-  if (blocks > 0x0fffffffLL) return fail(B200L_ERR_BAD_SHAPE, "kv_append: too many tokens and heads");
+  const int per = 8 / kv_append_group(DHP);      // groups of a block
+  const long long blocks = ((long long)a.windows * a.c.heads * 2 + per - 1) / per;
+  if (blocks > 0x7fffffffLL) return fail(B200L_ERR_BAD_SHAPE, "kv_append: too many tokens and heads");
   cudaError_t e = a.type == B200L_DTYPE_F32
                       ? launch_pdl(kv_append_kernel<DHP, KIND, 4>, dim3((unsigned)blocks), dim3(256), 0, st, a)
                       : launch_pdl(kv_append_kernel<DHP, KIND, 2>, dim3((unsigned)blocks), dim3(256), 0, st, a);
@@ -156,9 +157,11 @@ int kv_append_run(const b200l_kv_cache* cache, const b200l_kv_rows* rows, const 
   a.num_slots = cache->num_pages * cache->page_size;
   a.type = rows->dtype;
   a.dh = cache->head_dim;
-  // Windows of up to 64 tokens a warp, while there are 32 warps for every SM.
-  a.window = 1;
-  while (a.window < 64 && tokens * cache->num_heads * 2 / (a.window * 2) >= 32ll * dev.sms) a.window *= 2;
+  // Windows from a token per warp to 64 tokens a group, while there are 128
+  // warps for every SM.
+  const int gw = kv_append_group(kv_padded(a.dh));
+  a.window = gw;
+  while (a.window < 64 && tokens * cache->num_heads * 2 / (a.window * 2) * gw >= 128ll * dev.sms) a.window *= 2;
   a.windows = (int)((tokens + a.window - 1) / a.window);
 #define KV_CALL(D, K) kv_append_t<D, K>(a, st)
   KV_DISPATCH(cache->head_dim, cache->kind, KV_CALL)
@@ -253,7 +256,7 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
     const int mq = p->dhp == 256 ? 128 : 256, bn = p->dhp == 256 ? 64 : 128;
     p->M = mq;
     p->workers = 0;
-    a.row_tiles = a.min_pages = 0;
+    a.row_tiles = a.min_pages = a.whole = 0;
     p->tiles = (int)((long long)d->tokens * a.group / mq) + (d->requests < d->tokens ? d->requests : d->tokens);
     const long long items = (long long)p->tiles * cache->num_heads;
     // Few items: as many pieces along the keys as keep every SM busy, of at
@@ -265,11 +268,18 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
     p->pieces = p->splits > 1 ? items * p->splits : 0;
   } else {
     p->tiles = p->splits = 0;
-    p->M = rows > 16 && p->dhp <= 128 ? 32 : 16;
+    p->M = rows <= 8 ? 8 : rows <= 16 || p->dhp == 256 ? 16 : 32;
     a.row_tiles = rows > p->M ? (rows + p->M - 1) / p->M : 1;
     const int tk = p->dhp == 256 ? 16 : p->dhp == 128 ? 32 : 64;
     a.min_pages = 2 * tk > cache->page_size ? 2 * tk / cache->page_size : 1;
-    p->workers = dev.sms * (p->dhp == 256 || p->M == 32 ? 2 : 3) * 4;
+    // Up to four key tiles a pair: a warp is done with them sooner than two
+    // launches are (4 requests of 126 tokens, 4 heads of 32: 8.6 against 11.9 us).
+    a.whole = d->table_width * cache->page_size <= 4 * tk;
+    // Every SM full, but no more blocks than full tables would have work for.
+    const int full = dev.sms * (p->dhp * p->M >= 4096 || p->M == 32 ? 2 : 3);
+    const long long units = (long long)cache->num_heads * a.row_tiles * d->requests * d->table_width;
+    const long long blocks = (units + 4ll * a.min_pages - 1) / (4ll * a.min_pages);
+    p->workers = 4 * (int)(blocks < full ? blocks : full);
     p->pieces = 2ll * p->workers;
   }
   p->off_o = 1024;
@@ -279,9 +289,9 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
   return B200L_OK;
 }
 
-template <int DHP, int KIND, int MT>
+template <int DHP, int KIND, int NR>
 int kv_decode_t(KvAttnPlan& p, uint8_t* ws, cudaStream_t st) {
-  using C = KvDecCfg<DHP, MT>;
+  using C = KvDecCfg<DHP, NR>;
   KvAttnArgs& a = p.a;
   CUtensorMap mk, mv;
   const unsigned long long dims[2] = {(unsigned long long)DHP, (unsigned long long)(a.c.num_pages * a.c.heads * a.c.page)};
@@ -291,13 +301,13 @@ int kv_decode_t(KvAttnPlan& p, uint8_t* ws, cudaStream_t st) {
   int rc = make_map(&mk, a.c.k, 2, dims, strides, box, swz, "k codes", CU_TENSOR_MAP_DATA_TYPE_UINT8);
   if (rc) return rc;
   if ((rc = make_map(&mv, a.c.v, 2, dims, strides, box, swz, "v codes", CU_TENSOR_MAP_DATA_TYPE_UINT8))) return rc;
-  auto kern = kv_decode_kernel<DHP, KIND, MT>;
+  auto kern = kv_decode_kernel<DHP, KIND, NR>;
   if ((rc = ensure_smem((const void*)kern, C::SMEM))) return rc;
   const int grid = p.workers / C::WARPS;
   cudaError_t e = launch_pdl(kern, dim3(grid), dim3(128), C::SMEM, st, mk, mv, a, reinterpret_cast<DevStatus*>(ws));
   if (e != cudaSuccess) return cuda_fail(e, "kv_decode_kernel");
-  if ((rc = check_launch("kv_decode_kernel"))) return rc;
-  e = launch_pdl(kv_join_kernel<DHP>, dim3(p.workers), dim3(128), 0, st, a, p.workers, p.M);
+  if ((rc = check_launch("kv_decode_kernel")) || a.whole) return rc;
+  e = launch_pdl(kv_join_kernel<DHP>, dim3(p.workers), dim3(256), 0, st, a, p.workers, p.M);
   if (e != cudaSuccess) return cuda_fail(e, "kv_join_kernel");
   return check_launch("kv_join_kernel");
 }
@@ -357,17 +367,7 @@ int kv_attention_run(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, v
     KV_DISPATCH(cache->head_dim, cache->kind, KV_CALL)
 #undef KV_CALL
   }
-  if (p.M == 32) {
-    switch (p.dhp * 2 + cache->kind) {
-      case 64: return kv_decode_t<32, kKvInt8, 2>(p, w, st);
-      case 65: return kv_decode_t<32, kKvE4M3, 2>(p, w, st);
-      case 128: return kv_decode_t<64, kKvInt8, 2>(p, w, st);
-      case 129: return kv_decode_t<64, kKvE4M3, 2>(p, w, st);
-      case 256: return kv_decode_t<128, kKvInt8, 2>(p, w, st);
-      default: return kv_decode_t<128, kKvE4M3, 2>(p, w, st);
-    }
-  }
-#define KV_CALL(D, K) kv_decode_t<D, K, 1>(p, w, st)
+#define KV_CALL(D, K) (p.M == 8 ? kv_decode_t<D, K, 1>(p, w, st) : p.M == 16 ? kv_decode_t<D, K, 2>(p, w, st) : kv_decode_t<D, K, D == 256 ? 2 : 4>(p, w, st))
   KV_DISPATCH(cache->head_dim, cache->kind, KV_CALL)
 #undef KV_CALL
 }

@@ -52,10 +52,15 @@ __device__ __forceinline__ void codes4_to_half(uint32_t w, uint32_t& lo, uint32_
   }
 }
 
-__device__ __forceinline__ float load_elem(const void* p, long long i, int type) {
-  if (type == kElemF16) return __half2float(static_cast<const __half*>(p)[i]);
-  if (type == kElemBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return static_cast<const float*>(p)[i];
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t pack_elem2(float a, float b, int type) {

@@ -1,8 +1,8 @@
 // kv_decode.cuh -- attention of few rows per request over a paged 8-bit cache.
 //
 // A row is one query head of one new token; the rows of a request that share a
-// key/value head (new tokens x query heads per key head) are one tile of M = 16
-// or 32 rows, so the cache is read once for all of them. With codes c, scales
+// key/value head (new tokens x query heads per key head) are one tile of M = 8,
+// 16 or 32 rows, so the cache is read once for all of them. With codes c, scales
 // s_k, s_v per page and head, and key j visible to the row:
 //   t_j = log2(e) scale s_k(j) <q, c_k(j)>         u_j = t_j + log2 s_v(j)
 //   o   = sum_j 2^(u_j - M) c_v(j) / sum_j 2^(u_j - M) / s_v(j),   M = max u
@@ -22,14 +22,22 @@
 // 12 warps x 8-16 KB in flight cover HBM's latency several times over). A pair
 // that lies inside one stretch is finished there; of one that is cut, each
 // piece leaves (max, sum, accumulator) in the workspace and kv_join_kernel adds
-// them in order.
+// them in order (64 requests, 32 / 8 heads of 128: 5 us more; the last warp to
+// leave a piece adding them itself, 8 us). Where tables are too narrow for it to
+// be worth it, stretches are whole pairs and there is nothing to join.
 //
 // Products are mma.sync m16n8k16: one tile of M rows has too little work for
-// tcgen05 (2 FLOP per byte read and row; HBM bounds it below M ~ 250). Which
-// dims or keys a fragment's place stands for is free as long as both operands
-// agree, so fragments are read straight from the page's rows: as B of Q K^T a
-// lane takes 16 consecutive code bytes of its key; as B of P V the same bytes of
-// four keys, transposed by byte permutes on the way to fp16.
+// tcgen05 (2 FLOP per byte read and row; HBM bounds it below M ~ 250). The
+// transposed products are taken, S^T = K Q^T and O^T = V^T P^T, so that the 16
+// of the shape are keys or dims, always full, and the 8 are rows: a token's few
+// query heads pad to 8, and accumulators, Q and exponentials are half of what
+// 16-row tiles of Q K^T hold. Which dims or keys a fragment's place stands for is
+// free as long as both operands agree, so fragments are read straight from the
+// page's rows: as A of K Q^T a lane takes 16 consecutive code bytes of a key; as A
+// of V^T P^T the same bytes of four keys, transposed by byte permutes on the way
+// to fp16. P^T goes from accumulator to operand by movmatrix. The row sums are a
+// product with ones, of the weights as fp16 has them, so that what rounds a
+// weight rounds it above and below alike.
 #pragma once
 
 #include "kv_common.cuh"
@@ -48,11 +56,11 @@ struct KvAttnArgs {
   const int* cu_pages;
   float* part_o;                 // [2 * workers][M][dhp]
   float* part_ml;                // [2 * workers][M][2]
-  int requests, width, tokens, hq, group, dh, type, causal, row_tiles, min_pages, q_vec, q_vec8, o_vec8;
+  int requests, width, tokens, hq, group, dh, type, causal, row_tiles, min_pages, whole, q_vec, q_vec8, o_vec8;
   float scale_log2;              // softmax scale * log2(e)
 };
 
-template <int DHP, int MT>
+template <int DHP, int NR>       // rows of a tile: 8 NR
 struct KvDecCfg {
   static constexpr int TK = DHP == 256 ? 16 : DHP == 128 ? 32 : 64;   // keys of a tile
   static constexpr int ROWB = DHP < 128 ? DHP : 128;                  // bytes of a swizzled row
@@ -60,71 +68,106 @@ struct KvDecCfg {
   static constexpr int CODE = TK * DHP;                               // bytes of K (and of V) in a slot
   static constexpr int SLOTS = 2;
   static constexpr int WARPS = 4;
-  static constexpr bool QSM = DHP * MT > 128;                         // Q fragments in shared memory
-  static constexpr int QB = QSM ? MT * 16 * DHP * 2 : 0;
+  static constexpr bool QSM = DHP * NR >= 512;                        // Q fragments in shared memory
+  static constexpr int M = 8 * NR;
+  static constexpr int QB = QSM ? M * DHP * 2 : 0;
   static constexpr int SMEM = WARPS * (SLOTS * 2 * CODE + QB) + WARPS * SLOTS * 8 + WARPS * SLOTS * 4 * 8 + 64 + 1024;
-  static constexpr int CTAS = DHP == 256 || MT == 2 ? 2 : 3;            // resident per SM (registers)
-  static constexpr int M = 16 * MT;
+  static constexpr int CTAS = DHP * NR >= 512 || NR == 4 ? 2 : 3;     // resident per SM (registers)
 };
 
 // A warp's stretch of the pages of all (request, head, row tile) triples.
 struct KvSpan {
-  long long u, u1;
+  long long u, u1, stretch;      // pages of a stretch, but for the last
   int r, h, np, len, p0, p1;     // pages [p0, p1) of np; h counts (head, row tile)
+  int tok0, n;                   // the request's new tokens
+  int base;                      // cu_pages[r]
   bool done;
 
-  __device__ __forceinline__ void cut(const KvAttnArgs& a, int heads) {
+  __device__ __forceinline__ void cut(const KvAttnArgs& a) {
     const long long left = u1 - u;
-    p1 = (long long)(np - p0) < left ? np : p0 + (int)left;
-    len = min(max(a.lens[r], 0), min(np, a.width) << a.c.log2_page);
+    p1 = (long long)(np - p0) < left || a.whole ? np : p0 + (int)left;
   }
-  __device__ __forceinline__ void begin(const KvAttnArgs& a, int heads, long long from, long long to, int lane) {
-    u = from;
-    u1 = to;
-    done = u >= u1;
+  __device__ __forceinline__ int clip_len(const KvAttnArgs& a, int l) const {
+    return min(max(l, 0), min(np, a.width) << a.c.log2_page);
+  }
+  // Request r, from its five numbers at once.
+  __device__ __forceinline__ void open(const KvAttnArgs& a) {
+    const int c0 = a.cu_pages[r], c1 = a.cu_pages[r + 1], t0 = a.cu_new[r], t1 = a.cu_new[r + 1], l = a.lens[r];
+    base = c0;
+    np = c1 - c0;
+    tok0 = t0;
+    n = t1 - t0;
+    len = clip_len(a, l);
+  }
+  // The stretch of worker w, at the triple that it begins in, or with `last` at
+  // the one that holds the last page of a full stretch (done if there is none).
+  __device__ __forceinline__ void begin(const KvAttnArgs& a, int heads, int workers, int w, int lane, bool last = false) {
+    int cp = 0, cn = 0, l = 0;
+    const bool few = a.requests < 32;             // a lane holds what there is of a request: one round trip
+    if (few) {
+      cp = a.cu_pages[min(lane, a.requests)];
+      cn = a.cu_new[min(lane, a.requests)];
+      l = a.lens[min(lane, a.requests - 1)];
+    }
+    const int total = few ? __shfl_sync(0xffffffffu, cp, a.requests) : a.cu_pages[a.requests];
+    const long long units = (long long)heads * total;
+    const long long c = (units + workers - 1) / workers;
+    stretch = c < a.min_pages ? a.min_pages : c;
+    u = w * stretch;
+    u1 = units < u + stretch ? units : u + stretch;
+    done = u >= u1 || (last && u + stretch >= units);
     if (done) return;
-    r = warp_find_owner(a.cu_pages, a.requests, u / heads, lane);
-    const long long base = (long long)a.cu_pages[r];
-    np = (int)(a.cu_pages[r + 1] - base);
+    if (last) u = u1 - 1;
+    const long long x = u / heads;
+    if (few) {
+      r = __popc(__ballot_sync(0xffffffffu, lane < a.requests && (long long)cp <= x)) - 1;
+      base = __shfl_sync(0xffffffffu, cp, r);
+      np = __shfl_sync(0xffffffffu, cp, r + 1) - base;
+      tok0 = __shfl_sync(0xffffffffu, cn, r);
+      n = __shfl_sync(0xffffffffu, cn, r + 1) - tok0;
+      len = clip_len(a, __shfl_sync(0xffffffffu, l, r));
+    } else {
+      r = warp_find_owner(a.cu_pages, a.requests, x, lane);
+      open(a);
+    }
     if (np <= 0) {                                // (cu_pages is no prefix sum)
       done = true;
       return;
     }
-    const long long off = u - base * heads;
+    const long long off = u - (long long)base * heads;
     h = (int)(off / np);
     p0 = (int)(off - (long long)h * np);
-    cut(a, heads);
+    if (a.whole && p0 > 0) {                      // the pair is whose stretch holds its first page
+      u += np - p0;
+      p0 = 0;
+      done = u >= u1;
+      if (!done) step(a, heads, lane);
+    }
+    cut(a);
+  }
+  // On to the triple after this one.
+  __device__ __forceinline__ void step(const KvAttnArgs& a, int heads, int lane) {
+    if (++h == heads) {
+      h = 0;
+      const int after = base + np;
+      ++r;
+      if (r < a.requests) open(a);
+      if (r >= a.requests || np <= 0) {           // requests without new tokens
+        r = warp_find_owner(a.cu_pages, a.requests, after, lane);
+        open(a);
+        if (np <= 0) done = true;
+      }
+    }
   }
   __device__ __forceinline__ void next(const KvAttnArgs& a, int heads, int lane) {
     u += p1 - p0;
-    if (u >= u1) {
-      done = true;
-      return;
-    }
     p0 = 0;
-    if (++h == heads) {
-      h = 0;
-      const int base = a.cu_pages[r + 1];
-      np = ++r + 1 <= a.requests ? a.cu_pages[r + 1] - base : 0;
-      if (np <= 0) {
-        r = warp_find_owner(a.cu_pages, a.requests, base, lane);
-        np = a.cu_pages[r + 1] - a.cu_pages[r];
-        if (np <= 0) {
-          done = true;
-          return;
-        }
-      }
-    }
-    cut(a, heads);
+    done = u >= u1;
+    if (done) return;
+    step(a, heads, lane);
+    cut(a);
   }
 };
-
-// How the pages are cut: the stretch of worker w of `workers`.
-__device__ __forceinline__ long long kv_chunk(const KvAttnArgs& a, int heads, int workers) {
-  const long long units = (long long)heads * a.cu_pages[a.requests];
-  const long long c = (units + workers - 1) / workers;
-  return c < a.min_pages ? a.min_pages : c;
-}
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -133,13 +176,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-}
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+// Transposes an 8 x 8 tile of 16-bit values, two of a row a lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ void store_out(const KvAttnArgs& a, long long at, int d, float x, float y) {
@@ -154,16 +195,16 @@ __device__ __forceinline__ void store_out(const KvAttnArgs& a, long long at, int
   if (d + 1 < a.dh) o[d + 1] = (unsigned short)(w >> 16);
 }
 
-template <int DHP, int KIND, int MT>
-__global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
-    kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, KvAttnArgs a,
+template <int DHP, int KIND, int NR>
+__global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
+    kv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ KvAttnArgs a,
                      DevStatus* status) {
-  using C = KvDecCfg<DHP, MT>;
-  constexpr int TK = C::TK, NT = TK / 8, KS = DHP / 16, M = C::M;
+  using C = KvDecCfg<DHP, NR>;
+  constexpr int TK = C::TK, KT = TK / 16, KS = DHP / 16, M = C::M;
   constexpr int KB = DHP >= 64 ? 16 : 8;          // code bytes of a lane's key at a time
   constexpr int KC = DHP / (4 * KB);              // ... and how many times
   constexpr int VB = DHP / 8 < 16 ? DHP / 8 : 16; // the same for values
-  constexpr int ND = DHP / 8;                     // 8-dim tiles of the output
+  constexpr int ND = DHP / 16;                    // 16-dim tiles of the output
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -187,13 +228,12 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
   const int P = a.c.page, lp = a.c.log2_page, PB = P < TK ? P : TK;   // keys of a box
   const int heads = a.c.heads * a.row_tiles;
   const int workers = gridDim.x * C::WARPS, w = blockIdx.x * C::WARPS + warp;
-  const long long units = (long long)heads * a.cu_pages[a.requests];
-  const long long chunk = kv_chunk(a, heads, workers);
-  const long long u0 = w * chunk, u1 = units < u0 + chunk ? units : u0 + chunk;
+  KvSpan sp;
+  sp.begin(a, heads, workers, w, lane);
+  const long long u0 = sp.u;
 
   // ---- the loads, two tiles ahead
-  KvSpan ld;
-  ld.begin(a, heads, u0, u1, lane);
+  KvSpan ld = sp;
   int lkey = 0, lend = 0, entry = -1;
   auto fetch_entry = [&]() {                      // page of this lane's box in the tile at lkey
     const int k = lkey + lane * PB;
@@ -251,83 +291,97 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
 
   int used = 0;
   bool ok = true;
-  KvSpan sp;
-  for (sp.begin(a, heads, u0, u1, lane); !sp.done && ok; sp.next(a, heads, lane)) {
+  for (; !sp.done && ok; sp.next(a, heads, lane)) {
     const int head = sp.h / a.row_tiles, rt = sp.h - head * a.row_tiles;
-    const int tok0 = a.cu_new[sp.r], n = a.cu_new[sp.r + 1] - tok0, rows = n * a.group;
+    const int tok0 = sp.tok0, n = sp.n, rows = n * a.group;
     const int row0 = rt * M;
     const bool live = row0 < rows;                // (else: no such row tile for this request)
     const int kend = min(sp.p1 << lp, sp.len);
-    // ---- Q fragments, and how far each row sees
-    uint32_t qf[C::QSM ? 1 : MT][C::QSM ? 1 : KS][4];
-    int lim[MT][2], lim_min = kend;
-    float qs[MT][2];
-    long long oat[MT][2];
+    // ---- Q fragments (row g of 8), and of the rows 2t, 2t + 1 that this lane's
+    // scores and outputs belong to: how far they see, their factor, their place.
+    uint32_t qf[C::QSM ? 1 : NR][C::QSM ? 1 : KS][2];
+    int lim[NR][2], lim_min = kend;
+    float qs[NR][2];
+    long long oat[NR][2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < NR; ++m) {
+      const int row = row0 + m * 8 + g, i = row / a.group, hq = head * a.group + row - i * a.group;
+      const bool in = row < rows && tok0 + i < a.tokens;
+      const void* q = a.q;
+      const long long at = (long long)(tok0 + i) * a.q_st + (long long)hq * a.q_sh;
+      uint32_t v[KS][2];
+      float big = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = row0 + m * 16 + g + 8 * e;
-        const int i = row / a.group, hq = head * a.group + row - i * a.group;
-        const bool in = row < rows && tok0 + i < a.tokens;
-        oat[m][e] = in ? ((long long)(tok0 + i) * a.hq + hq) * a.dh : -1;
-        lim[m][e] = in ? min(kend, a.causal ? sp.len - n + i + 1 : kend) : 0;
-        if (in) lim_min = min(lim_min, lim[m][e]);
-        const void* q = a.q;
-        const long long at = (long long)(tok0 + i) * a.q_st + (long long)hq * a.q_sh;
-        float v[KS][4], big = 0.f;
+      for (int s = 0; s < KS; ++s) {
+        // dims of k-step s: piece s / (KB / 4) of the row, then 4 of the lane's KB
+        constexpr int PER = KB / 4;
+        const int c = s / PER, d = (DHP <= 64 ? KB * t : 128 * (c / 2) + 32 * t + 16 * (c & 1)) + 4 * (s % PER);
+        if (in && a.q_vec && d + 4 <= a.dh) {
+          const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(q) + at + d);
+          v[s][0] = u.x;
+          v[s][1] = u.y;
+        } else {
+          const unsigned short* p = static_cast<const unsigned short*>(q) + at;
+          uint32_t e[4];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          // dims of k-step s: chunk s / (KB/4), then 4 of the lane's KB
-          constexpr int PER = KB / 4;
-          const int c = s / PER, d = (DHP == 32 ? KB * t : DHP == 64 ? KB * t : 128 * (c / 2) + 32 * t + 16 * (c & 1)) + 4 * (s % PER);
-          if (in && a.q_vec && d + 4 <= a.dh) {
-            const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(q) + at + d);
-            if (a.type == kElemF16) {
-              const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-              v[s][0] = x.x; v[s][1] = x.y; v[s][2] = y.x; v[s][3] = y.y;
-            } else {
-              const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x)), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-              v[s][0] = x.x; v[s][1] = x.y; v[s][2] = y.x; v[s][3] = y.y;
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[s][k] = in && d + k < a.dh ? load_elem(q, at + d + k, a.type) : 0.f;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) big = fmaxf(big, fabsf(v[s][k]));
+          for (int k = 0; k < 4; ++k) e[k] = in && d + k < a.dh ? p[d + k] : 0u;
+          v[s][0] = e[0] | e[1] << 16;
+          v[s][1] = e[2] | e[3] << 16;
         }
+      }
+      float f = a.scale_log2;
+      if (a.type == kElemBF16) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v[s][k]));
+            big = fmax3f(big, fabsf(x.x), fabsf(x.y));
+          }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         float mul = 1.f;
-        qs[m][e] = a.scale_log2;
-        big = quad_max(big);
-        if (a.type == kElemBF16 && big > 0.f && big < INFINITY) {
+        if (big > 0.f && big < INFINITY) {
           const int ex = min(max(((__float_as_int(big) >> 23) & 255) - 127, -120), 120);
           mul = __int_as_float((127 - ex) << 23);
-          qs[m][e] *= __int_as_float((127 + ex) << 23);
+          f *= __int_as_float((127 + ex) << 23);
         }
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const uint32_t x = pack_half2(v[s][0] * mul, v[s][1] * mul), y = pack_half2(v[s][2] * mul, v[s][3] * mul);
-          if constexpr (C::QSM) {
-            uint32_t* f = reinterpret_cast<uint32_t*>(qsm) + ((m * KS + s) * 32 + lane) * 4;
-            f[e] = x;
-            f[2 + e] = y;
-          } else {
-            qf[m][s][e] = x;
-            qf[m][s][2 + e] = y;
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v[s][k]));
+            v[s][k] = pack_half2(x.x * mul, x.y * mul);
           }
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if constexpr (C::QSM) {
+          *reinterpret_cast<uint2*>(qsm + ((m * KS + s) * 32 + lane) * 8) = make_uint2(v[s][0], v[s][1]);
+        } else {
+          qf[m][s][0] = v[s][0];
+          qf[m][s][1] = v[s][1];
         }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qs[m][e] = __shfl_sync(0xffffffffu, f, 8 * t + 4 * e);
+        const int r2 = row0 + m * 8 + 2 * t + e, i2 = r2 / a.group;
+        const bool in2 = r2 < rows && tok0 + i2 < a.tokens;
+        oat[m][e] = in2 ? ((long long)(tok0 + i2) * a.hq + head * a.group + r2 - i2 * a.group) * a.dh : -1;
+        lim[m][e] = in2 ? min(kend, a.causal ? sp.len - n + i2 + 1 : kend) : 0;
+        if (in2) lim_min = min(lim_min, lim[m][e]);
       }
     }
     lim_min = __reduce_min_sync(0xffffffffu, lim_min);
 
-    float o[MT][ND][4], mx[MT][2], l[MT][2];
+    float o[ND][NR][4], mx[NR][2], l[NR][2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < NR; ++m) {
       mx[m][0] = mx[m][1] = -INFINITY;
       l[m][0] = l[m][1] = 0.f;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[m][d][0] = o[m][d][1] = o[m][d][2] = o[m][d][3] = 0.f;
+      for (int d = 0; d < ND; ++d) o[d][m][0] = o[d][m][1] = o[d][m][2] = o[d][m][3] = 0.f;
     }
 
     for (int key = sp.p0 << lp; key < kend; key += TK) {
@@ -340,44 +394,50 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
       __syncwarp();
       const uint8_t* ks = ring + s * 2 * C::CODE;
       const uint8_t* vs = ks + C::CODE;
-      // ---- scores of 8 keys a tile
-      float acc[MT][NT][4];
+      // ---- scores, 16 keys x 8 rows a tile: keys g, g + 8, rows 2t, 2t + 1
+      float acc[KT][NR][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
+      for (int j = 0; j < KT; ++j) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
-        const int row = 8 * j + g;
+        for (int m = 0; m < NR; ++m) acc[j][m][0] = acc[j][m][1] = acc[j][m][2] = acc[j][m][3] = 0.f;
+      }
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          uint32_t wd[KB / 4];
-          if constexpr (DHP == 32) {
-            // 32-byte rows, 32B swizzle: 16-byte chunk ^= address bit 7
-            const uint2 u = *reinterpret_cast<const uint2*>(ks + row * 32 + ((((t >> 1) ^ (row >> 2)) & 1) << 4) + ((t & 1) << 3));
-            wd[0] = u.x;
-            wd[1] = u.y;
-          } else {
-            const uint8_t* p;
-            if constexpr (DHP == 64) p = ks + swz_offset(row, t, 64);
-            else p = ks + (c / 2) * TK * 128 + swz_offset(row, 2 * t + (c & 1), 128);
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            wd[0] = u.x;
-            wd[1] = u.y;
-            wd[2] = u.z;
-            wd[3] = u.w;
+      for (int c = 0; c < KC; ++c) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          uint32_t wd[2][KB / 4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = 16 * j + g + 8 * e;
+            if constexpr (DHP == 32) {
+              // 32-byte rows, 32B swizzle: 16-byte chunk ^= address bit 7
+              const uint2 u = *reinterpret_cast<const uint2*>(ks + row * 32 + ((((t >> 1) ^ (row >> 2)) & 1) << 4) + ((t & 1) << 3));
+              wd[e][0] = u.x;
+              wd[e][1] = u.y;
+            } else {
+              const uint8_t* p;
+              if constexpr (DHP == 64) p = ks + swz_offset(row, t, 64);
+              else p = ks + (c / 2) * TK * 128 + swz_offset(row, 2 * t + (c & 1), 128);
+              const uint4 u = *reinterpret_cast<const uint4*>(p);
+              wd[e][0] = u.x;
+              wd[e][1] = u.y;
+              wd[e][2] = u.z;
+              wd[e][3] = u.w;
+            }
           }
 #pragma unroll
           for (int i = 0; i < KB / 4; ++i) {
-            uint32_t b0, b1;
-            codes4_to_half<KIND>(wd[i], b0, b1);
+            uint32_t ka[4];
+            codes4_to_half<KIND>(wd[0][i], ka[0], ka[2]);
+            codes4_to_half<KIND>(wd[1][i], ka[1], ka[3]);
             const int st = c * (KB / 4) + i;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+            for (int m = 0; m < NR; ++m) {
               if constexpr (C::QSM) {
-                const uint4 u = *reinterpret_cast<const uint4*>(qsm + ((m * KS + st) * 32 + lane) * 16);
-                const uint32_t f[4] = {u.x, u.y, u.z, u.w};
-                mma_f16(acc[m][j], f, b0, b1);
+                const uint2 u = *reinterpret_cast<const uint2*>(qsm + ((m * KS + st) * 32 + lane) * 8);
+                mma_f16(acc[j][m], ka, u.x, u.y);
               } else {
-                mma_f16(acc[m][j], qf[m][st], b0, b1);
+                mma_f16(acc[j][m], ka, qf[m][st][0], qf[m][st][1]);
               }
             }
           }
@@ -386,52 +446,53 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
       // ---- u = t + log2 s_v, row maxima
       const int nbox = (min(kend - key, TK) + PB - 1) / PB;
       bool hole = key + TK > lim_min;
-      float inv[NT];
+      float inv[KT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int box = min(8 * j / PB, nbox - 1);
-        const float2 sc = scl[s * 4 + box];
+      for (int j = 0; j < KT; ++j) {
+        const float2 sc = scl[s * 4 + min(16 * j / PB, nbox - 1)];
         // A scale of 0 (a page of zeros) has no logarithm: 2^-100 stands for it.
         const float sv = fmaxf(sc.y, 7.8886090522101181e-31f);
-        const float lv = sc.y == sc.y ? __log2f(sv) : sc.y;
-        inv[j] = sv < INFINITY ? __fdividef(1.0f, sv) : 0.f;
-        const bool none = sc.y < 0.f;
-        hole |= none;
+        const float lv = sc.y == sc.y ? lg2_approx(sv) : sc.y;
+        inv[j] = sv < INFINITY ? rcp_approx(sv) : 0.f;
+        hole |= sc.y < 0.f;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < NR; ++m) {
           const float c0 = qs[m][0] * sc.x, c1 = qs[m][1] * sc.x;
-          acc[m][j][0] = fmaf(acc[m][j][0], c0, lv);
-          acc[m][j][1] = fmaf(acc[m][j][1], c0, lv);
-          acc[m][j][2] = fmaf(acc[m][j][2], c1, lv);
-          acc[m][j][3] = fmaf(acc[m][j][3], c1, lv);
+          acc[j][m][0] = fmaf(acc[j][m][0], c0, lv);
+          acc[j][m][1] = fmaf(acc[j][m][1], c1, lv);
+          acc[j][m][2] = fmaf(acc[j][m][2], c0, lv);
+          acc[j][m][3] = fmaf(acc[j][m][3], c1, lv);
         }
       }
       if (hole) {                                 // (warp-uniform)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const bool none = scl[s * 4 + min(8 * j / PB, nbox - 1)].y < 0.f;
-          const int k = key + 8 * j + 2 * t;
+        for (int j = 0; j < KT; ++j) {
+          const bool none = scl[s * 4 + min(16 * j / PB, nbox - 1)].y < 0.f;
+          const int k = key + 16 * j + g;
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            if (none || k >= lim[m][0]) acc[m][j][0] = -INFINITY;
-            if (none || k + 1 >= lim[m][0]) acc[m][j][1] = -INFINITY;
-            if (none || k >= lim[m][1]) acc[m][j][2] = -INFINITY;
-            if (none || k + 1 >= lim[m][1]) acc[m][j][3] = -INFINITY;
+          for (int m = 0; m < NR; ++m) {
+            if (none || k >= lim[m][0]) acc[j][m][0] = -INFINITY;
+            if (none || k >= lim[m][1]) acc[j][m][1] = -INFINITY;
+            if (none || k + 8 >= lim[m][0]) acc[j][m][2] = -INFINITY;
+            if (none || k + 8 >= lim[m][1]) acc[j][m][3] = -INFINITY;
           }
         }
       }
       // ---- weights; the accumulators move to a new maximum when it is 2^8 over the old
-      uint32_t p[MT][NT][2];
+      uint32_t p[KT][NR][2];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        float top0 = -INFINITY, top1 = -INFINITY;
+      for (int m = 0; m < NR; ++m) {
+        float top0 = fmaxf(acc[0][m][0], acc[0][m][2]), top1 = fmaxf(acc[0][m][1], acc[0][m][3]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          top0 = fmax3f(top0, acc[m][j][0], acc[m][j][1]);
-          top1 = fmax3f(top1, acc[m][j][2], acc[m][j][3]);
+        for (int j = 1; j < KT; ++j) {
+          top0 = fmax3f(top0, acc[j][m][0], acc[j][m][2]);
+          top1 = fmax3f(top1, acc[j][m][1], acc[j][m][3]);
         }
-        top0 = quad_max(top0);
-        top1 = quad_max(top1);
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) {
+          top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, x));
+          top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, x));
+        }
         const bool up0 = top0 > mx[m][0] + 8.f, up1 = top1 > mx[m][1] + 8.f;
         if (__any_sync(0xffffffffu, up0 || up1)) {
           const float a0 = up0 ? ex2_approx(mx[m][0] - top0) : 1.f, a1 = up1 ? ex2_approx(mx[m][1] - top1) : 1.f;
@@ -441,32 +502,33 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
           l[m][1] *= a1;
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            o[m][d][0] *= a0;
-            o[m][d][1] *= a0;
-            o[m][d][2] *= a1;
-            o[m][d][3] *= a1;
+            o[d][m][0] *= a0;
+            o[d][m][1] *= a1;
+            o[d][m][2] *= a0;
+            o[d][m][3] *= a1;
           }
         }
         const float m0 = mx[m][0] == -INFINITY ? 0.f : mx[m][0], m1 = mx[m][1] == -INFINITY ? 0.f : mx[m][1];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float x0 = ex2_approx(acc[m][j][0] - m0), x1 = ex2_approx(acc[m][j][1] - m0);
-          const float x2 = ex2_approx(acc[m][j][2] - m1), x3 = ex2_approx(acc[m][j][3] - m1);
-          l[m][0] = fmaf(x0 + x1, inv[j], l[m][0]);
-          l[m][1] = fmaf(x2 + x3, inv[j], l[m][1]);
-          p[m][j][0] = pack_half2(x0, x1);
-          p[m][j][1] = pack_half2(x2, x3);
+        for (int j = 0; j < KT; ++j) {
+          p[j][m][0] = transpose8x8(pack_half2(ex2_approx(acc[j][m][0] - m0), ex2_approx(acc[j][m][1] - m1)));
+          p[j][m][1] = transpose8x8(pack_half2(ex2_approx(acc[j][m][2] - m0), ex2_approx(acc[j][m][3] - m1)));
+          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16(sum, ones, p[j][m][0], p[j][m][1]);
+          l[m][0] = fmaf(sum[0], inv[j], l[m][0]);
+          l[m][1] = fmaf(sum[1], inv[j], l[m][1]);
         }
       }
-      // ---- O += P V, 16 keys a step
+      // ---- O^T += V^T P^T, 16 keys a step
 #pragma unroll
-      for (int i = 0; i < NT / 2; ++i) {
+      for (int j = 0; j < KT; ++j) {
 #pragma unroll
         for (int hb = 0; hb < C::NH; ++hb) {
           uint32_t kw[4][VB / 4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int row = 16 * i + 2 * t + (k & 1) + 8 * (k >> 1);
+            const int row = 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
             if constexpr (DHP == 32) {
               kw[k][0] = *reinterpret_cast<const uint32_t*>(vs + row * 32 + ((((g >> 2) ^ (row >> 2)) & 1) << 4) + ((g & 3) << 2));
             } else if constexpr (DHP == 64) {
@@ -480,7 +542,11 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
               kw[k][2] = u.z;
               kw[k][3] = u.w;
             }
-            if (hole) {                           // what lies past the keys is not read as a number
+          }
+          if (hole) {                             // what lies past the keys is not read as a number
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
               const bool none = row + key >= kend || scl[s * 4 + min(row / PB, nbox - 1)].y < 0.f;
 #pragma unroll
               for (int b = 0; b < VB / 4; ++b) kw[k][b] = none ? 0u : kw[k][b];
@@ -491,17 +557,15 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
             // bytes of four keys for four dims -> per dim the pairs (keys 0, 1) and (2, 3)
             const uint32_t x01 = __byte_perm(kw[0][b], kw[1][b], 0x5140), y01 = __byte_perm(kw[0][b], kw[1][b], 0x7362);
             const uint32_t x23 = __byte_perm(kw[2][b], kw[3][b], 0x5140), y23 = __byte_perm(kw[2][b], kw[3][b], 0x7362);
-            uint32_t f01[4], f23[4];
-            codes4_to_half<KIND>(x01, f01[0], f01[1]);
-            codes4_to_half<KIND>(y01, f01[2], f01[3]);
-            codes4_to_half<KIND>(x23, f23[0], f23[1]);
-            codes4_to_half<KIND>(y23, f23[2], f23[3]);
+            uint32_t va[2][4];
+            codes4_to_half<KIND>(x01, va[0][0], va[0][1]);
+            codes4_to_half<KIND>(x23, va[0][2], va[0][3]);
+            codes4_to_half<KIND>(y01, va[1][0], va[1][1]);
+            codes4_to_half<KIND>(y23, va[1][2], va[1][3]);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const uint32_t pa[4] = {p[m][2 * i][0], p[m][2 * i][1], p[m][2 * i + 1][0], p[m][2 * i + 1][1]};
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-              for (int d = 0; d < 4; ++d) mma_f16(o[m][hb * 16 + 4 * b + d], pa, f01[d], f23[d]);
-            }
+              for (int m = 0; m < NR; ++m) mma_f16(o[hb * 8 + 2 * b + e][m], va[e], p[j][m][0], p[j][m][1]);
           }
         }
       }
@@ -511,42 +575,47 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
     }
     if (!ok) break;
 
-    // ---- the pair's result, or this piece of it
+    // ---- the pair's result, or this piece of it: dims [VB g, VB g + VB) of each box
     const bool whole = sp.p0 == 0 && sp.p1 == sp.np;
     // Pieces: slot 2w holds the one that the stretch begins with, 2w + 1 the one that it ends with.
     const long long slot = 2ll * w + (sp.u == u0 ? 0 : 1);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < NR; ++m) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float lt = quad_sum(l[m][e]);
         if (!live || oat[m][e] < 0) continue;
-        const int row = m * 16 + g + 8 * e;
-        if (whole) {
-          const float r = lt == 0.f ? 0.f : 1.0f / lt;
+        const int row = m * 8 + 2 * t + e;
+        const float lt = l[m][e], r = lt == 0.f ? 0.f : 1.0f / lt;
+        if (!whole && g == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * M + row) * 2) = make_float2(mx[m][e], lt);
 #pragma unroll
-          for (int hb = 0; hb < C::NH; ++hb)
+        for (int hb = 0; hb < C::NH; ++hb) {
+          const int d0 = hb * 128 + VB * g;
+          if (whole) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int d = 0; d < VB; d += 2)
+              store_out(a, oat[m][e], d0 + d, o[hb * 8 + d / 2][m][e] * r, o[hb * 8 + d / 2][m][2 + e] * r);
+          } else {
 #pragma unroll
-              for (int d = 0; d < VB; d += 2)
-                store_out(a, oat[m][e], hb * 128 + VB * (2 * t + c) + d, o[m][hb * 16 + d][2 * e + c] * r,
-                          o[m][hb * 16 + d + 1][2 * e + c] * r);
-        } else {
-          float* po = a.part_o + (slot * M + row) * DHP;
-          if (t == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * M + row) * 2) = make_float2(mx[m][e], lt);
-#pragma unroll
-          for (int hb = 0; hb < C::NH; ++hb)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int d = 0; d < VB; d += 4)
-                *reinterpret_cast<float4*>(po + hb * 128 + VB * (2 * t + c) + d) =
-                    make_float4(o[m][hb * 16 + d][2 * e + c], o[m][hb * 16 + d + 1][2 * e + c],
-                                o[m][hb * 16 + d + 2][2 * e + c], o[m][hb * 16 + d + 3][2 * e + c]);
+            for (int d = 0; d < VB; d += 4)
+              *reinterpret_cast<float4*>(a.part_o + (slot * M + row) * DHP + d0 + d) =
+                  make_float4(o[hb * 8 + d / 2][m][e], o[hb * 8 + d / 2][m][2 + e], o[hb * 8 + d / 2 + 1][m][e],
+                              o[hb * 8 + d / 2 + 1][m][2 + e]);
+          }
         }
       }
     }
+  }
+  // Rows that attend to nothing: of requests without keys, and past the plan's tokens.
+  {
+    auto zero_rows = [&](int t0, int t1) {
+      const long long e1 = (long long)min(t1, a.tokens) * a.hq * a.dh;
+      for (long long i = (long long)t0 * a.hq * a.dh + lane; i < e1; i += 32) static_cast<unsigned short*>(a.out)[i] = 0;
+    };
+    for (int r = w; r < a.requests; r += workers) {
+      const int c0 = a.cu_pages[r], c1 = a.cu_pages[r + 1], t0 = a.cu_new[r], t1 = a.cu_new[r + 1];
+      if (c0 == c1 && t1 > t0) zero_rows(t0, t1);
+    }
+    for (int i = a.cu_new[a.requests] + w; i < a.tokens; i += workers) zero_rows(i, i + 1);
   }
   if (!ok) {                                      // copies in flight land before the block goes
     for (int i = used; i < issued; ++i) mbar_drain(&bars[i & 1], (i >> 1) & 1);
@@ -558,70 +627,86 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, MT>::CTAS)
 
 // Joins the pieces of every pair that was cut, in order: with M = max m_i,
 // o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i. A block per worker looks
-// whether a pair begins in that worker's stretch and goes on past it; warps
-// take its rows. Also zeroes the rows that attend to nothing: those of requests
-// without keys, and those past the plan's tokens.
+// whether a pair begins in that worker's stretch and goes on past it; its
+// threads take 4 dims of a row each and, where rows are few, every so many'th
+// piece.
 template <int DHP>
-__global__ void __launch_bounds__(128) kv_join_kernel(KvAttnArgs a, int workers, int M) {
+__global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ KvAttnArgs a, int workers, int M) {
   pdl_wait_then_release();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gw = blockIdx.x * 4 + warp, nw = gridDim.x * 4;
-  auto zero_rows = [&](int t0, int t1) {
-    const long long e1 = (long long)min(t1, a.tokens) * a.hq * a.dh;
-    for (long long i = (long long)t0 * a.hq * a.dh + lane; i < e1; i += 32) static_cast<unsigned short*>(a.out)[i] = 0;
-  };
-  for (int r = gw; r < a.requests; r += nw)
-    if (a.cu_pages[r + 1] == a.cu_pages[r] && a.cu_new[r + 1] > a.cu_new[r]) zero_rows(a.cu_new[r], a.cu_new[r + 1]);
-  for (int i = a.cu_new[a.requests] + gw; i < a.tokens; i += nw) zero_rows(i, i + 1);
-
+  __shared__ float2 s_row[32];                    // maximum, 1 / sum
+  __shared__ float4 s_acc[256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = blockIdx.x;
   const int heads = a.c.heads * a.row_tiles;
-  const long long units = (long long)heads * a.cu_pages[a.requests];
-  const long long chunk = kv_chunk(a, heads, workers);
-  const int w = blockIdx.x;
-  const long long u0 = w * chunk, u1 = u0 + chunk;
-  if (u1 >= units) return;                        // nothing lies past this stretch
-  // The pair that holds the stretch's last page.
-  const int r = warp_find_owner(a.cu_pages, a.requests, (u1 - 1) / heads, lane);
-  const long long base = (long long)heads * a.cu_pages[r];
-  const int np = a.cu_pages[r + 1] - a.cu_pages[r];
-  if (np <= 0) return;
-  const int h = (int)((u1 - 1 - base) / np);
-  const long long b = base + (long long)h * np, e = b + np;
+  KvSpan sp;
+  sp.begin(a, heads, workers, w, lane, true);
+  if (sp.done) return;                            // nothing lies past this stretch
+  const long long u0 = w * sp.stretch, u1 = u0 + sp.stretch;
+  const long long b = sp.u - sp.p0, e = b + sp.np;
   if (b < u0 || e <= u1) return;                  // begins earlier, or ends here
-  const int pieces = (int)((e - 1) / chunk) - w + 1;
-  const int head = h / a.row_tiles, rt = h - head * a.row_tiles;
-  const int tok0 = a.cu_new[r], rows = (a.cu_new[r + 1] - tok0) * a.group;
+  const int pieces = (int)((e - 1) / sp.stretch) - w + 1;
+  const int head = sp.h / a.row_tiles, row0 = (sp.h - head * a.row_tiles) * M;
+  const int tok0 = sp.tok0;
+  const int rows = min(M, min(sp.n, a.tokens - tok0) * a.group - row0);
+  if (rows <= 0) return;
   auto slot = [&](int i) { return i == 0 && b != u0 ? 2ll * w + 1 : 2ll * (w + i); };
-  for (int row = warp; row < M; row += 4) {
-    const int gr = rt * M + row, i = gr / a.group;
-    if (gr >= rows || tok0 + i >= a.tokens) break;
-    float top = -INFINITY;
-    for (int k = lane; k < pieces; k += 32) top = fmaxf(top, a.part_ml[(slot(k) * M + row) * 2]);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    if (top == -INFINITY) top = 0.f;
-    constexpr int PER = DHP / 32;
-    float acc[PER], l = 0.f;
-#pragma unroll
-    for (int d = 0; d < PER; ++d) acc[d] = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < pieces; ++k) {
-      const long long at = slot(k) * M + row;
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-      const float f = ex2_approx(ml.x - top);
-      l = fmaf(ml.y, f, l);
-#pragma unroll
-      for (int d = 0; d < PER; ++d) acc[d] = fmaf(a.part_o[at * DHP + d * 32 + lane], f, acc[d]);
+  for (int row = warp; row < rows; row += 8) {
+    float top = -INFINITY, l = 0.f;
+    for (int k = lane; k < pieces; k += 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot(k) * M + row) * 2);
+      const float m = fmaxf(top, ml.x), m0 = m == -INFINITY ? 0.f : m;
+      l = l * ex2_approx(top - m0) + ml.y * ex2_approx(ml.x - m0);
+      top = m;
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const long long at = ((long long)(tok0 + i) * a.hq + head * a.group + gr - i * a.group) * a.dh;
 #pragma unroll
-    for (int d = 0; d < PER; ++d) {
-      const int dim = d * 32 + lane;
-      if (dim < a.dh) {
-        if (a.type == kElemF16) static_cast<__half*>(a.out)[at + dim] = __float2half_rn(acc[d] * inv);
-        else static_cast<__nv_bfloat16*>(a.out)[at + dim] = __float2bfloat16_rn(acc[d] * inv);
+    for (int s = 16; s > 0; s >>= 1) {
+      const float t2 = __shfl_xor_sync(0xffffffffu, top, s), l2 = __shfl_xor_sync(0xffffffffu, l, s);
+      const float m = fmaxf(top, t2), m0 = m == -INFINITY ? 0.f : m;
+      l = l * ex2_approx(top - m0) + l2 * ex2_approx(t2 - m0);
+      top = m;
+    }
+    if (lane == 0) s_row[row] = make_float2(top == -INFINITY ? 0.f : top, l == 0.f ? 0.f : 1.0f / l);
+  }
+  __syncthreads();
+  constexpr int LN = DHP / 4, GROUPS = 256 / LN;
+  int rp = 1;
+  while (rp < rows && rp < GROUPS) rp *= 2;
+  const int split = GROUPS / rp;
+  const int q = threadIdx.x / LN, d = (threadIdx.x % LN) * 4, mine = q % rp, part = q / rp;
+  for (int r0 = 0; r0 < rows; r0 += rp) {
+    const int row = r0 + mine;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < rows) {
+      const float top = s_row[row].x;
+#pragma unroll 8
+      for (int k = part; k < pieces; k += split) {
+        const long long at = slot(k) * M + row;
+        const float f = ex2_approx(a.part_ml[at * 2] - top);
+        const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * DHP + d);
+        acc.x = fmaf(o.x, f, acc.x);
+        acc.y = fmaf(o.y, f, acc.y);
+        acc.z = fmaf(o.z, f, acc.z);
+        acc.w = fmaf(o.w, f, acc.w);
       }
+    }
+    if (split > 1) {
+      __syncthreads();
+      s_acc[threadIdx.x] = acc;
+      __syncthreads();
+      if (part == 0)
+        for (int p = 1; p < split; ++p) {
+          const float4 o = s_acc[threadIdx.x + p * rp * LN];
+          acc.x += o.x;
+          acc.y += o.y;
+          acc.z += o.z;
+          acc.w += o.w;
+        }
+    }
+    if (part == 0 && row < rows) {
+      const float inv = s_row[row].y;
+      const int gr = row0 + row, i = gr / a.group;
+      const long long at = ((long long)(tok0 + i) * a.hq + head * a.group + gr - i * a.group) * a.dh;
+      store_out(a, at, d, acc.x * inv, acc.y * inv);
+      store_out(a, at, d + 2, acc.z * inv, acc.w * inv);
     }
   }
 }

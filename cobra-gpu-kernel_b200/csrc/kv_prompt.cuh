@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
             const float svc = fmaxf(sv, 7.8886090522101181e-31f);      // 2^-100 for a page of zeros
             float4 c;
             c.x = sk;
-            c.y = !there ? -INFINITY : sv == sv ? __log2f(svc) : sv;
-            c.z = !there || !(svc < INFINITY) ? 0.f : __fdividef(1.0f, svc);
+            c.y = !there ? -INFINITY : sv == sv ? lg2_approx(svc) : sv;
+            c.z = !there || !(svc < INFINITY) ? 0.f : rcp_approx(svc);
             c.w = there ? 1.f : 0.f;
             for (int i = 0; i < PB / 16; ++i) consts[cs * (GR + 1) + lane * (PB / 16) + i] = c;
           }

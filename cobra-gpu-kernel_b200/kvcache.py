@@ -174,7 +174,11 @@ class _Workspace:
         for (index, stream), held in self._held.items():
             with torch.cuda.device(index):
                 for ptr, _, _ in held:
-                    _lib.check(_lib.lib().b200l_read_status(ptr, stream))
+                    rc = _lib.lib().b200l_read_status(ptr, stream)
+                    if rc:
+                        message = _lib.last_error()
+                        _lib.lib().b200l_clear_status(ptr, stream)
+                        raise _lib.B200LError(rc, message)
 
 
 _workspace = _Workspace()

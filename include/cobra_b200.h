@@ -384,8 +384,10 @@ typedef struct b200l_kv_attn_desc {
     float scale;
 } b200l_kv_attn_desc;
 
-/* Workspace bytes (1024-byte aligned; status block first: b200l_clear_status
- * before its first use, b200l_read_status). 0 for a bad shape. */
+/* Workspace bytes (1024-byte aligned; 0 for a bad shape). The status block comes
+ * first: b200l_clear_status before the workspace's first use and after a
+ * recorded failure, b200l_read_status. Calls that may overlap need a workspace
+ * each. */
 B200L_API size_t b200l_kv_attention_workspace_bytes(const b200l_kv_cache* cache, const b200l_kv_attn_desc* desc);
 B200L_API int b200l_kv_attention(const b200l_kv_cache* cache, const b200l_kv_attn_desc* desc, void* workspace,
                                  size_t ws_bytes, void* stream);
