@@ -256,7 +256,7 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
     const int mq = p->dhp == 256 ? 128 : 256, bn = p->dhp == 256 ? 64 : 128;
     p->M = mq;
     p->workers = 0;
-    a.row_tiles = a.min_pages = a.whole = 0;
+    a.row_tiles = a.min_units = a.whole = a.log2_unit = 0;
     p->tiles = (int)((long long)d->tokens * a.group / mq) + (d->requests < d->tokens ? d->requests : d->tokens);
     const long long items = (long long)p->tiles * cache->num_heads;
     // Few items: as many pieces along the keys as keep every SM busy, of at
@@ -271,14 +271,16 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
     p->M = rows <= 8 ? 8 : rows <= 16 || p->dhp == 256 ? 16 : 32;
     a.row_tiles = rows > p->M ? (rows + p->M - 1) / p->M : 1;
     const int tk = p->dhp == 256 ? 16 : p->dhp == 128 ? 32 : 64;
-    a.min_pages = 2 * tk > cache->page_size ? 2 * tk / cache->page_size : 1;
+    const int unit = cache->page_size < tk ? cache->page_size : tk;
+    a.log2_unit = unit == 16 ? 4 : unit == 32 ? 5 : 6;
+    a.min_units = 2 * tk / unit;
     // Up to four key tiles a pair: a warp is done with them sooner than two
     // launches are (4 requests of 126 tokens, 4 heads of 32: 8.6 against 11.9 us).
     a.whole = d->table_width * cache->page_size <= 4 * tk;
     // Every SM full, but no more blocks than full tables would have work for.
     const int full = dev.sms * (p->dhp * p->M >= 4096 || p->M == 32 ? 2 : 3);
-    const long long units = (long long)cache->num_heads * a.row_tiles * d->requests * d->table_width;
-    const long long blocks = (units + 4ll * a.min_pages - 1) / (4ll * a.min_pages);
+    const long long units = (long long)cache->num_heads * a.row_tiles * d->requests * d->table_width * (cache->page_size / unit);
+    const long long blocks = (units + 4ll * a.min_units - 1) / (4ll * a.min_units);
     p->workers = 4 * (int)(blocks < full ? blocks : full);
     p->pieces = 2ll * p->workers;
   }
@@ -318,18 +320,6 @@ int kv_prompt_t(const KvAttnPlan& p, uint8_t* ws, cudaStream_t st) {
   auto kern = kv_prompt_kernel<DHP, KIND>;
   int rc = ensure_smem((const void*)kern, C::SMEM);
   if (rc) return rc;
-  if (C::NQ == 2) {
-    // The warps share out the registers of the launch: fewer than planned for, and they would wait for ever.
-    static std::atomic<int> regs{0};
-    if (!regs.load()) {
-      cudaFuncAttributes fa;
-      cudaError_t e = cudaFuncGetAttributes(&fa, (const void*)kern);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(kv_prompt_kernel)");
-      regs.store(fa.numRegs);
-    }
-    if (regs.load() < C::R_LAUNCH)
-      return fail(B200L_ERR_LAUNCH, "kv_prompt_kernel was built with %d registers, its shares need %d", regs.load(), C::R_LAUNCH);
-  }
   DevInfo dev;
   if ((rc = device_info(&dev))) return rc;
   KvPromptArgs pa;

@@ -14,7 +14,7 @@
 // if it comes as bf16: exact but for what is 2^-14 of it) and the weights.
 //
 // Bound: HBM, 2 dhp bytes per cached token and head. Work is split evenly over
-// warps, not requests: the pages of all (request, head) pairs in a row are cut
+// warps, not requests: the keys of all (request, head) pairs in a row are cut
 // into one stretch per warp, so 2 requests of 100000 tokens and 256 of a
 // thousand fill the GPU alike, and warps never wait for one another. A warp
 // streams its stretch through two slots of its own shared memory (TMA, one box
@@ -56,7 +56,7 @@ struct KvAttnArgs {
   const int* cu_pages;
   float* part_o;                 // [2 * workers][M][dhp]
   float* part_ml;                // [2 * workers][M][2]
-  int requests, width, tokens, hq, group, dh, type, causal, row_tiles, min_pages, whole, q_vec, q_vec8, o_vec8;
+  int requests, width, tokens, hq, group, dh, type, causal, row_tiles, min_units, whole, log2_unit, q_vec, q_vec8, o_vec8;
   float scale_log2;              // softmax scale * log2(e)
 };
 
@@ -75,33 +75,35 @@ struct KvDecCfg {
   static constexpr int CTAS = DHP * NR >= 512 || NR == 4 ? 2 : 3;     // resident per SM (registers)
 };
 
-// A warp's stretch of the pages of all (request, head, row tile) triples.
+// A warp's stretch of the keys of all (request, head, row tile) triples, in
+// units of 2^log2_unit keys: a page, or a key tile of one where that is less.
 struct KvSpan {
-  long long u, u1, stretch;      // pages of a stretch, but for the last
-  int r, h, np, len, p0, p1;     // pages [p0, p1) of np; h counts (head, row tile)
+  long long u, u1, stretch;      // units of a stretch, but for the last
+  int r, head, rt, nu, len, p0, p1;   // units [p0, p1) of nu, of request r's key head and row tile
   int tok0, n;                   // the request's new tokens
   int base;                      // cu_pages[r]
   bool done;
 
   __device__ __forceinline__ void cut(const KvAttnArgs& a) {
     const long long left = u1 - u;
-    p1 = (long long)(np - p0) < left || a.whole ? np : p0 + (int)left;
+    p1 = (long long)(nu - p0) < left || a.whole ? nu : p0 + (int)left;
   }
-  __device__ __forceinline__ int clip_len(const KvAttnArgs& a, int l) const {
-    return min(max(l, 0), min(np, a.width) << a.c.log2_page);
+  __device__ __forceinline__ void set(const KvAttnArgs& a, int c0, int c1, int t0, int t1, int l) {
+    const int np = c1 - c0;
+    base = c0;
+    nu = np << (a.c.log2_page - a.log2_unit);
+    tok0 = t0;
+    n = t1 - t0;
+    len = min(max(l, 0), min(np, a.width) << a.c.log2_page);
   }
   // Request r, from its five numbers at once.
   __device__ __forceinline__ void open(const KvAttnArgs& a) {
     const int c0 = a.cu_pages[r], c1 = a.cu_pages[r + 1], t0 = a.cu_new[r], t1 = a.cu_new[r + 1], l = a.lens[r];
-    base = c0;
-    np = c1 - c0;
-    tok0 = t0;
-    n = t1 - t0;
-    len = clip_len(a, l);
+    set(a, c0, c1, t0, t1, l);
   }
   // The stretch of worker w, at the triple that it begins in, or with `last` at
-  // the one that holds the last page of a full stretch (done if there is none).
-  __device__ __forceinline__ void begin(const KvAttnArgs& a, int heads, int workers, int w, int lane, bool last = false) {
+  // the one that holds the last unit of a full stretch (done if there is none).
+  __device__ __forceinline__ void begin(const KvAttnArgs& a, int workers, int w, int lane, bool last = false) {
     int cp = 0, cn = 0, l = 0;
     const bool few = a.requests < 32;             // a lane holds what there is of a request: one round trip
     if (few) {
@@ -110,61 +112,63 @@ struct KvSpan {
       l = a.lens[min(lane, a.requests - 1)];
     }
     const int total = few ? __shfl_sync(0xffffffffu, cp, a.requests) : a.cu_pages[a.requests];
-    const long long units = (long long)heads * total;
+    const long long per = (long long)a.c.heads * a.row_tiles << (a.c.log2_page - a.log2_unit);   // units of a page
+    const long long units = per * total;
     const long long c = (units + workers - 1) / workers;
-    stretch = c < a.min_pages ? a.min_pages : c;
+    stretch = c < a.min_units ? a.min_units : c;
     u = w * stretch;
     u1 = units < u + stretch ? units : u + stretch;
     done = u >= u1 || (last && u + stretch >= units);
     if (done) return;
     if (last) u = u1 - 1;
-    const long long x = u / heads;
+    const long long x = u / per;
     if (few) {
       r = __popc(__ballot_sync(0xffffffffu, lane < a.requests && (long long)cp <= x)) - 1;
-      base = __shfl_sync(0xffffffffu, cp, r);
-      np = __shfl_sync(0xffffffffu, cp, r + 1) - base;
-      tok0 = __shfl_sync(0xffffffffu, cn, r);
-      n = __shfl_sync(0xffffffffu, cn, r + 1) - tok0;
-      len = clip_len(a, __shfl_sync(0xffffffffu, l, r));
+      const int c0 = __shfl_sync(0xffffffffu, cp, r), c1 = __shfl_sync(0xffffffffu, cp, r + 1);
+      const int t0 = __shfl_sync(0xffffffffu, cn, r), t1 = __shfl_sync(0xffffffffu, cn, r + 1);
+      set(a, c0, c1, t0, t1, __shfl_sync(0xffffffffu, l, r));
     } else {
       r = warp_find_owner(a.cu_pages, a.requests, x, lane);
       open(a);
     }
-    if (np <= 0) {                                // (cu_pages is no prefix sum)
+    if (nu <= 0) {                                // (cu_pages is no prefix sum)
       done = true;
       return;
     }
-    const long long off = u - (long long)base * heads;
-    h = (int)(off / np);
-    p0 = (int)(off - (long long)h * np);
-    if (a.whole && p0 > 0) {                      // the pair is whose stretch holds its first page
-      u += np - p0;
+    const long long off = u - base * per;
+    const int h = (int)(off / nu);
+    p0 = (int)(off - (long long)h * nu);
+    head = h / a.row_tiles;
+    rt = h - head * a.row_tiles;
+    if (a.whole && p0 > 0) {                      // the pair is whose stretch holds its first unit
+      u += nu - p0;
       p0 = 0;
       done = u >= u1;
-      if (!done) step(a, heads, lane);
+      if (!done) step(a, lane);
     }
     cut(a);
   }
   // On to the triple after this one.
-  __device__ __forceinline__ void step(const KvAttnArgs& a, int heads, int lane) {
-    if (++h == heads) {
-      h = 0;
-      const int after = base + np;
-      ++r;
-      if (r < a.requests) open(a);
-      if (r >= a.requests || np <= 0) {           // requests without new tokens
-        r = warp_find_owner(a.cu_pages, a.requests, after, lane);
-        open(a);
-        if (np <= 0) done = true;
-      }
+  __device__ __forceinline__ void step(const KvAttnArgs& a, int lane) {
+    if (++rt < a.row_tiles) return;
+    rt = 0;
+    if (++head < a.c.heads) return;
+    head = 0;
+    const int after = base + (nu >> (a.c.log2_page - a.log2_unit));
+    ++r;
+    if (r < a.requests) open(a);
+    if (r >= a.requests || nu <= 0) {             // requests without new tokens
+      r = warp_find_owner(a.cu_pages, a.requests, after, lane);
+      open(a);
+      if (nu <= 0) done = true;
     }
   }
-  __device__ __forceinline__ void next(const KvAttnArgs& a, int heads, int lane) {
+  __device__ __forceinline__ void next(const KvAttnArgs& a, int lane) {
     u += p1 - p0;
     p0 = 0;
     done = u >= u1;
     if (done) return;
-    step(a, heads, lane);
+    step(a, lane);
     cut(a);
   }
 };
@@ -225,11 +229,11 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
   }
   __syncthreads();
 
-  const int P = a.c.page, lp = a.c.log2_page, PB = P < TK ? P : TK;   // keys of a box
-  const int heads = a.c.heads * a.row_tiles;
+  // Keys of a box: a page, or a tile of it (the unit of the cuts, if not a smaller page).
+  const int P = a.c.page, lp = a.c.log2_page, lb = a.log2_unit, PB = 1 << lb;
   const int workers = gridDim.x * C::WARPS, w = blockIdx.x * C::WARPS + warp;
   KvSpan sp;
-  sp.begin(a, heads, workers, w, lane);
+  sp.begin(a, workers, w, lane);
   const long long u0 = sp.u;
 
   // ---- the loads, two tiles ahead
@@ -241,10 +245,10 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
   };
   auto open_span = [&]() {                        // on to the next stretch that has keys
     while (!ld.done) {
-      lkey = ld.p0 << lp;
-      lend = min(ld.p1 << lp, ld.len);
+      lkey = ld.p0 << lb;
+      lend = min(ld.p1 << lb, ld.len);
       if (lkey < lend) break;
-      ld.next(a, heads, lane);
+      ld.next(a, lane);
     }
     if (!ld.done) fetch_entry();
   };
@@ -254,14 +258,13 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
     if (!ld.done) {
       const int s = issued & 1;
       const bool ok = entry >= 0 && entry < a.c.num_pages;
-      const int head = ld.h / a.row_tiles;
       const unsigned boxes = __ballot_sync(0xffffffffu, ok);
       if (lane == 0) mbar_arrive_expect_tx(&bars[s], (uint32_t)__popc(boxes) * 2u * (uint32_t)(PB * DHP));
       __syncwarp();
       if (lane * PB < TK) {
         if (ok) {
-          const long long ph = (long long)entry * a.c.heads + head;
-          const int row = (int)((ph << lp) + ((lkey + lane * PB) & (P - 1)));
+          const int ph = entry * a.c.heads + ld.head;     // (rows of the cache stay below 2^31)
+          const int row = (ph << lp) + ((lkey + lane * PB) & (P - 1));
           uint8_t* kd = ring + s * 2 * C::CODE + lane * PB * C::ROWB;
 #pragma unroll
           for (int b = 0; b < C::NH; ++b) {
@@ -278,7 +281,7 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
       ++issued;
       lkey += TK;
       if (lkey >= lend) {
-        ld.next(a, heads, lane);
+        ld.next(a, lane);
         open_span();
       } else {
         fetch_entry();
@@ -291,12 +294,12 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
 
   int used = 0;
   bool ok = true;
-  for (; !sp.done && ok; sp.next(a, heads, lane)) {
-    const int head = sp.h / a.row_tiles, rt = sp.h - head * a.row_tiles;
+  for (; !sp.done && ok; sp.next(a, lane)) {
+    const int head = sp.head, rt = sp.rt;
     const int tok0 = sp.tok0, n = sp.n, rows = n * a.group;
     const int row0 = rt * M;
     const bool live = row0 < rows;                // (else: no such row tile for this request)
-    const int kend = min(sp.p1 << lp, sp.len);
+    const int kend = min(sp.p1 << lb, sp.len);
     // ---- Q fragments (row g of 8), and of the rows 2t, 2t + 1 that this lane's
     // scores and outputs belong to: how far they see, their factor, their place.
     uint32_t qf[C::QSM ? 1 : NR][C::QSM ? 1 : KS][2];
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
       for (int d = 0; d < ND; ++d) o[d][m][0] = o[d][m][1] = o[d][m][2] = o[d][m][3] = 0.f;
     }
 
-    for (int key = sp.p0 << lp; key < kend; key += TK) {
+    for (int key = sp.p0 << lb; key < kend; key += TK) {
       const int s = used & 1;
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       if (!mbar_wait_warp(&bars[s], (used >> 1) & 1, wc)) {
@@ -444,12 +447,12 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
         }
       }
       // ---- u = t + log2 s_v, row maxima
-      const int nbox = (min(kend - key, TK) + PB - 1) / PB;
+      const int nbox = (min(kend - key, TK) + PB - 1) >> lb;
       bool hole = key + TK > lim_min;
       float inv[KT];
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
-        const float2 sc = scl[s * 4 + min(16 * j / PB, nbox - 1)];
+        const float2 sc = scl[s * 4 + min((16 * j) >> lb, nbox - 1)];
         // A scale of 0 (a page of zeros) has no logarithm: 2^-100 stands for it.
         const float sv = fmaxf(sc.y, 7.8886090522101181e-31f);
         const float lv = sc.y == sc.y ? lg2_approx(sv) : sc.y;
@@ -467,7 +470,7 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
       if (hole) {                                 // (warp-uniform)
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-          const bool none = scl[s * 4 + min(16 * j / PB, nbox - 1)].y < 0.f;
+          const bool none = scl[s * 4 + min((16 * j) >> lb, nbox - 1)].y < 0.f;
           const int k = key + 16 * j + g;
 #pragma unroll
           for (int m = 0; m < NR; ++m) {
@@ -547,7 +550,7 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int row = 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
-              const bool none = row + key >= kend || scl[s * 4 + min(row / PB, nbox - 1)].y < 0.f;
+              const bool none = row + key >= kend || scl[s * 4 + min(row >> lb, nbox - 1)].y < 0.f;
 #pragma unroll
               for (int b = 0; b < VB / 4; ++b) kw[k][b] = none ? 0u : kw[k][b];
             }
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
     if (!ok) break;
 
     // ---- the pair's result, or this piece of it: dims [VB g, VB g + VB) of each box
-    const bool whole = sp.p0 == 0 && sp.p1 == sp.np;
+    const bool whole = sp.p0 == 0 && sp.p1 == sp.nu;
     // Pieces: slot 2w holds the one that the stretch begins with, 2w + 1 the one that it ends with.
     const long long slot = 2ll * w + (sp.u == u0 ? 0 : 1);
 #pragma unroll
@@ -636,15 +639,14 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ Kv
   __shared__ float2 s_row[32];                    // maximum, 1 / sum
   __shared__ float4 s_acc[256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = blockIdx.x;
-  const int heads = a.c.heads * a.row_tiles;
   KvSpan sp;
-  sp.begin(a, heads, workers, w, lane, true);
+  sp.begin(a, workers, w, lane, true);
   if (sp.done) return;                            // nothing lies past this stretch
   const long long u0 = w * sp.stretch, u1 = u0 + sp.stretch;
-  const long long b = sp.u - sp.p0, e = b + sp.np;
+  const long long b = sp.u - sp.p0, e = b + sp.nu;
   if (b < u0 || e <= u1) return;                  // begins earlier, or ends here
   const int pieces = (int)((e - 1) / sp.stretch) - w + 1;
-  const int head = sp.h / a.row_tiles, row0 = (sp.h - head * a.row_tiles) * M;
+  const int head = sp.head, row0 = sp.rt * M;
   const int tok0 = sp.tok0;
   const int rows = min(M, min(sp.n, a.tokens - tok0) * a.group - row0);
   if (rows <= 0) return;

@@ -16,8 +16,12 @@
 // raw scores (c >= 0) and the row sum is corrected once per 16 weights.
 //
 // Warps: 0 loads pages and scales, 1 issues S of both tiles, 2 / 3 issue P V of
-// tile 0 / 1, 4-7 convert, 8.. are the softmax (eight per tile, 16 rows a warp,
-// two threads per row with half the keys each). P goes back to TMEM as fp16: in
+// tile 0 / 1, 4-7 convert, 8.. are the softmax: eight per tile, 16 rows a warp,
+// two threads per row with half the keys each, so that each scheduler has four of
+// them in turn at loads, maxima and exponentials. 80 registers a thread hold 32
+// scores: the first 32 are read for their maximum, the second kept, and the first
+// read again.
+// P goes back to TMEM as fp16: in
 // its own columns where they suffice (dhp <= 64, and dhp 256 with one tile), so
 // that the next S is computed meanwhile; over S at dhp 128, where two O and two
 // S fill TMEM and the tiles alternate instead. O is rescaled only when a row's
@@ -61,13 +65,10 @@ struct KvPromptCfg {
   static constexpr int P_STEP = OVER ? 128 : 64;
   static constexpr int O_COL = DHP <= 64 ? 384 : 256;
   static constexpr int O_STEP = DHP <= 64 ? 64 : 128;
-  // Registers of the three kinds of warps (setmaxnreg); together what the
-  // launch holds: 768 threads of 80.
-  static constexpr int R_LAUNCH = 80, R_ISSUE = 40, R_CONV = 56, R_SOFT = 96;
+  // Columns of P's 16-key groups: one after another, or over S at the place of
+  // the first of every 32 scores, so that none is overwritten that is still read.
+  __host__ __device__ static constexpr int p_col(int k) { return OVER ? 64 * (k >> 2) + 32 * ((k >> 1) & 1) + 8 * (k & 1) : 8 * k; }
 };
-static_assert(128 * (KvPromptCfg<128>::R_ISSUE + KvPromptCfg<128>::R_CONV) + 512 * KvPromptCfg<128>::R_SOFT ==
-                  768 * KvPromptCfg<128>::R_LAUNCH,
-              "the register shares add up to the launch's");
 
 // A work item: rows [row0, row0 + MQ) of request r for key head h, key tiles [j0, j1).
 struct KvItem {
@@ -122,10 +123,14 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// The barrier that every warp ends on. Each kind of warp has its own, and never
+// meets the others' code again, so that its register count is its own too.
+__device__ __forceinline__ void block_end() { asm volatile("bar.sync 0;" ::: "memory"); }
+
 template <int DHP, int KIND>
 __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel(KvPromptArgs p, DevStatus* status) {
   using C = KvPromptCfg<DHP>;
-  constexpr int BN = C::BN, GR = C::GR, HC = BN / 2;
+  constexpr int BN = C::BN, GR = C::GR, NP = BN / 64;   // pieces of 32 keys a thread
   const KvAttnArgs& a = p.a;
   pdl_wait_then_release();
   extern __shared__ uint8_t smem_raw[];
@@ -135,7 +140,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
   uint8_t* sV = sK + 2 * C::KV_BYTES;
   uint8_t* c8K = sV + 2 * C::KV_BYTES;
   uint8_t* c8V = c8K + C::ST8 * C::C_BYTES;
-  float4* consts = reinterpret_cast<float4*>(c8V + C::ST8 * C::C_BYTES);   // [CSLOTS][GR + 1]; the last: .x = whole
+  float4* consts = reinterpret_cast<float4*>(c8V + C::ST8 * C::C_BYTES);   // [CSLOTS][GR + 1]; the last: .x whole, .y poisoned
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(consts) + C::SM_CONST);
   uint64_t* q_full = bars;          // [2]
   uint64_t* q_empty = bars + 2;     // [2]
@@ -190,7 +195,6 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
   const int P = a.c.page, lp = a.c.log2_page, PB = P < BN ? P : BN;
 
   if (warp < 4) {
-    if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_ISSUE));
     if (warp == 0) {  // ================= pages and scales
       int g = 0, gk = 0, gv = 0;                  // tiles; K and V copies begun
       bool ok = true;
@@ -217,18 +221,26 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
           __syncwarp();
           if (there) bulk_load(c8K + s8 * C::C_BYTES + lane * PB * DHP, a.c.k + src, PB * DHP, &k8_full[s8]);
           ++gk;
+          bool poison = false;
           // The constants of this lane's keys, 16 at a time.
           if (lane * PB < BN) {
+            // w: 0 no such page, 1 a page, 2 one whose scales are no numbers: its visible
+            // scores become not-a-number, its constants are finite.
+            const bool fine = sk - sk == 0.f && sv - sv == 0.f;
             const float svc = fmaxf(sv, 7.8886090522101181e-31f);      // 2^-100 for a page of zeros
             float4 c;
-            c.x = sk;
-            c.y = !there ? -INFINITY : sv == sv ? lg2_approx(svc) : sv;
-            c.z = !there || !(svc < INFINITY) ? 0.f : rcp_approx(svc);
-            c.w = there ? 1.f : 0.f;
+            c.x = fine ? sk : 0.f;
+            c.y = !there ? -INFINITY : fine ? lg2_approx(svc) : 0.f;
+            c.z = !there ? 0.f : fine ? rcp_approx(svc) : 1.f;
+            c.w = !there ? 0.f : fine ? 1.f : 2.f;
+            poison = there && !fine;
             for (int i = 0; i < PB / 16; ++i) consts[cs * (GR + 1) + lane * (PB / 16) + i] = c;
           }
           const int want = min(BN / PB, (it.len - j * BN + PB - 1) / PB);
-          if (lane == 0) consts[cs * (GR + 1) + GR].x = (int)boxes >= want && (j + 1) * BN <= it.len ? 1.f : 0.f;
+          poison = __any_sync(0xffffffffu, poison);
+          if (lane == 0)
+            *reinterpret_cast<float2*>(&consts[cs * (GR + 1) + GR]) =
+                make_float2((int)boxes >= want && (j + 1) * BN <= it.len ? 1.f : 0.f, poison ? 1.f : 0.f);
           __syncwarp();
           if (lane == 0) mbar_arrive(&c_full[cs]);
           if (!mbar_wait_warp(&v8_free[s8], parity, wc)) { ok = false; break; }
@@ -241,6 +253,8 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       // Copies in flight land before the block goes (each stage's last one).
       for (int i = max(0, gk - C::ST8); i < gk; ++i) mbar_drain(&k8_full[i % C::ST8], (i / C::ST8) & 1);
       for (int i = max(0, gv - C::ST8); i < gv; ++i) mbar_drain(&v8_full[i % C::ST8], (i / C::ST8) & 1);
+      block_end();
+      if (lane == 0 && waitctl_aborted(wc)) record_error(status, -7, kKernelKvPrompt, 1);
     } else if (warp == 1) {  // ================= S_t(j) = Q_t K_j^T
       const uint32_t idesc_s = idesc_f16_f32(128, BN);
       const uint64_t dq0 = sdesc_kmajor(smem_u32(sQ), C::ROWB);
@@ -284,6 +298,9 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
         umma_commit(mma_done);
         mbar_drain(mma_done, 0);
       }
+      block_end();
+      tc_fence_after();
+      tmem_dealloc(tmem_base, 512);
     } else if (warp - 2 < C::NQ) {  // ================= O_t += P_t(j) V_j
       const int t = warp - 2;
       const uint32_t idesc_o = idesc_f16_f32(128, DHP) | (1u << 16);       // B is MN-major
@@ -309,7 +326,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < BN / 16; ++k)
-              umma_f16_ts(d_o, a_p + k * 8, dv + ((uint32_t)(k * 16 * C::ROWB) >> 4), idesc_o, k > 0 ? 1u : acc0);
+              umma_f16_ts(d_o, a_p + C::p_col(k), dv + ((uint32_t)(k * 16 * C::ROWB) >> 4), idesc_o, k > 0 ? 1u : acc0);
             umma_commit(&pv_done[t]);
             umma_commit(&v_empty[st]);
             ++np;
@@ -321,9 +338,12 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
         umma_commit(mma_done);
         mbar_drain(mma_done, 0);
       }
+      block_end();
+    } else {
+      block_end();
     }
+    return;
   } else if (warp < 8) {  // ================= codes -> fp16
-    if constexpr (C::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_CONV));
     const int tid = threadIdx.x - 128;
     constexpr int UPR = DHP / 16;                 // 16-code pieces of a row
     constexpr int UNITS = BN * UPR / 128;         // ... of a thread
@@ -384,17 +404,16 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
         }
       }
     }
+    block_end();
+    return;
   } else {  // ================= softmax
-    if constexpr (C::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFT));
-    const int sw = warp - 8, t = sw >> 3, hh = (sw >> 2) & 1, qd = warp & 3;
-    const int c = lane >> 4;                      // key half, and dim half, of this thread
-    const int row = qd * 32 + hh * 16 + (lane & 15);
-    const uint32_t lane_off = (uint32_t)(qd * 32 + hh * 16) << 16;
+    const int sw = warp - 8, t = sw >> 3, hh = (sw >> 2) & 1, c = lane >> 4;   // c: which half of the keys, and dims
+    const int row = (warp & 3) * 32 + hh * 16 + (lane & 15);
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32 + hh * 16) << 16;
     const uint32_t t_s = tmem_base + lane_off + C::S_COL + t * 128;
     const uint32_t t_p = tmem_base + lane_off + C::P_COL + t * C::P_STEP;
     const uint32_t t_o = tmem_base + lane_off + C::O_COL + t * C::O_STEP;
     constexpr int OH = DHP / 2;                   // dims of this thread
-    constexpr int OC = OH < 32 ? OH : 32;         // ... at a time
     int g = 0, ns = 0, np = 0, qi = 0;
     bool ok = true;
     // Rows past the plan's tokens.
@@ -414,105 +433,118 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       const int lim = !in ? 0 : a.causal ? min(it.len, it.len - it.n + i + 1) : it.len;
       const int first = (it.row0 + t * 128) / a.group;              // the tile's first token sees least
       const int lim_min = a.causal ? min(it.len, it.len - it.n + first + 1) : it.len;
+      const long long oat = ((long long)(it.tok0 + i) * a.hq + hq) * a.dh;
+      const int jbeg = it.j0, jend = it.j1;
       float qs = a.scale_log2, m_use = 0.f, l = 0.f;
       bool none = true;                           // no visible key so far
-      if (it.j0 < it.j1) {  // ---- Q_t as fp16, scaled by a power of two if it comes as bf16
-        const long long at = (long long)(it.tok0 + i) * a.q_st + (long long)hq * a.q_sh + c * OH;
-        uint32_t w[OH / 2];
-        if (in && a.q_vec8 && (c + 1) * OH <= a.dh) {
+      if (jbeg < jend) {  // ---- the row of Q as fp16, scaled by a power of two if it comes as bf16
+        const long long at = (long long)(it.tok0 + i) * a.q_st + (long long)hq * a.q_sh;
+        const uint4* q8 = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + at);
+        const unsigned short* q1 = static_cast<const unsigned short*>(a.q) + at;
+        auto load8 = [&](int d) {                 // dims [d, d + 8)
+          if (in && a.q_vec8 && d + 8 <= a.dh) return q8[d / 8];
+          uint32_t w[4];
 #pragma unroll
-          for (int d = 0; d < OH / 8; ++d) {
-            const uint4 u = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + at)[d];
-            w[4 * d] = u.x;
-            w[4 * d + 1] = u.y;
-            w[4 * d + 2] = u.z;
-            w[4 * d + 3] = u.w;
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t x = in && d + 2 * k < a.dh ? q1[d + 2 * k] : 0u;
+            const uint32_t y = in && d + 2 * k + 1 < a.dh ? q1[d + 2 * k + 1] : 0u;
+            w[k] = x | y << 16;
           }
-        } else {
-          const unsigned short* q = static_cast<const unsigned short*>(a.q) + at;
-#pragma unroll
-          for (int d = 0; d < OH / 2; ++d) {
-            const int d0 = c * OH + 2 * d;
-            const uint32_t x = in && d0 < a.dh ? q[2 * d] : 0u, y = in && d0 + 1 < a.dh ? q[2 * d + 1] : 0u;
-            w[d] = x | y << 16;
-          }
-        }
+          return make_uint4(w[0], w[1], w[2], w[3]);
+        };
+        float mul = 1.f;
         if (a.type == kElemBF16) {
           float big = 0.f;
+#pragma unroll 4
+          for (int d = 0; d < OH; d += 8) {
+            const uint4 u = load8(c * OH + d);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-          for (int d = 0; d < OH / 2; ++d) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[d]));
-            big = fmax3f(big, fabsf(f.x), fabsf(f.y));
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+              big = fmax3f(big, fabsf(f.x), fabsf(f.y));
+            }
           }
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
-          float mul = 1.f;
           if (big > 0.f && big < INFINITY) {
             const int ex = min(max(((__float_as_int(big) >> 23) & 255) - 127, -120), 120);
             mul = __int_as_float((127 - ex) << 23);
             qs *= __int_as_float((127 + ex) << 23);
           }
-#pragma unroll
-          for (int d = 0; d < OH / 2; ++d) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[d]));
-            w[d] = pack_half2(f.x * mul, f.y * mul);
-          }
         }
         if (!mbar_wait_warp(&q_empty[t], (qi & 1) ^ 1, wc)) { ok = false; break; }
         ++qi;
         const uint32_t dst = smem_u32(sQ + t * C::Q_BYTES);
+#pragma unroll 4
+        for (int d = 0; d < OH; d += 8) {
+          const uint4 u = load8(c * OH + d);
+          uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          if (a.type == kElemBF16) {
 #pragma unroll
-        for (int d = 0; d < OH / 8; ++d) {
-          const int chunk = c * (OH / 8) + d;     // 8 dims
-          st_shared_v4(dst + (chunk / (C::ROWB / 16)) * 128 * C::ROWB + swz_offset(row, chunk % (C::ROWB / 16), C::ROWB),
-                       w[4 * d], w[4 * d + 1], w[4 * d + 2], w[4 * d + 3]);
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+              w[k] = pack_half2(f.x * mul, f.y * mul);
+            }
+          }
+          const int chunk = (c * OH + d) / 8;
+          st_shared_v4(dst + (chunk / (C::ROWB / 16)) * 128 * C::ROWB + swz_offset(row, chunk % (C::ROWB / 16), C::ROWB), w[0],
+                       w[1], w[2], w[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[t]);
       }
-      for (int j = it.j0; j < it.j1; ++j, ++g) {
+      for (int j = jbeg; j < jend; ++j, ++g) {
         const int cs = g % C::CSLOTS;
         if (!mbar_wait_warp(&c_full[cs], (g / C::CSLOTS) & 1, wc) || !mbar_wait_warp(&s_full[t], ns & 1, wc)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        float s[HC];
-        {
-          uint32_t r[HC];
-          tmem_ld_pair32<HC>(t_s, *reinterpret_cast<uint32_t(*)[32]>(r));
-          if constexpr (HC == 64) tmem_ld_pair32<HC>(t_s + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
-#pragma unroll
-          for (int k = 0; k < HC; ++k) s[k] = __uint_as_float(r[k]);
-        }
-        tc_fence_before();
-        if constexpr (!C::OVER) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[t]);
-        }
-        ++ns;
-        const int kv0 = j * BN + HC * c;          // first key of this thread's half
-        const bool edge = (j + 1) * BN > lim_min; // (warp-uniform)
-        if (edge) {
-#pragma unroll
-          for (int k = 0; k < HC; ++k)
-            if (kv0 + k >= lim) s[k] = -INFINITY;
-        }
+        // This thread's keys: 32 NP from BN/2 c on, in pieces of 32.
         const float4* cc = consts + cs * (GR + 1) + c * (GR / 2);
-        float cg[HC / 16], lg[HC / 16], ig[HC / 16], hm = -INFINITY;
+        const bool edge = (j + 1) * BN > lim_min; // (warp-uniform)
+        const bool poison = consts[cs * (GR + 1) + GR].y != 0.f;
+        float s[32];
+        auto load = [&](int h) {
+          tmem_ld_pair32<BN / 2>(t_s + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(s));
+          if (edge) {
+            const int left = lim - (j * BN + (BN / 2) * c + 32 * h);
 #pragma unroll
-        for (int q = 0; q < HC / 16; ++q) {
-          const float4 k4 = cc[q];
-          cg[q] = k4.x * qs;
-          lg[q] = k4.y;
-          ig[q] = k4.z;
-          float m0 = fmaxf(s[16 * q], s[16 * q + 1]), m1 = fmaxf(s[16 * q + 2], s[16 * q + 3]);
-#pragma unroll
-          for (int k = 4; k < 16; k += 4) {
-            m0 = fmax3f(m0, s[16 * q + k], s[16 * q + k + 1]);
-            m1 = fmax3f(m1, s[16 * q + k + 2], s[16 * q + k + 3]);
+            for (int k = 0; k < 32; ++k)
+              if (k >= left) s[k] = -INFINITY;
           }
-          hm = fmaxf(hm, fmaf(fmaxf(m0, m1), cg[q], lg[q]));
+          if (poison) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              if (cc[2 * h + q].w == 2.f) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if (s[16 * q + k] != -INFINITY) s[16 * q + k] = __int_as_float(0x7fc00000);
+              }
+          }
+        };
+        // (A factor is above 0, so that hidden keys stay hidden: -inf * 0 is no number.)
+        auto top = [&](int h) {
+          float m[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float2 k2 = *reinterpret_cast<const float2*>(cc + 2 * h + q);
+            float m0 = fmaxf(s[16 * q], s[16 * q + 1]), m1 = fmaxf(s[16 * q + 2], s[16 * q + 3]);
+#pragma unroll
+            for (int k = 4; k < 16; k += 4) {
+              m0 = fmax3f(m0, s[16 * q + k], s[16 * q + k + 1]);
+              m1 = fmax3f(m1, s[16 * q + k + 2], s[16 * q + k + 3]);
+            }
+            m[q] = fmaf(fmaxf(m0, m1), fmaxf(k2.x * qs, 1e-37f), k2.y);
+          }
+          return fmaxf(m[0], m[1]);
+        };
+        load(0);
+        float hm = top(0);
+        if constexpr (NP == 2) {
+          load(1);
+          hm = fmaxf(hm, top(1));
         }
         const float m_cand = fmaxf(hm, __shfl_xor_sync(0xffffffffu, hm, 16));
         float alpha = 1.f;
@@ -527,47 +559,59 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
           m_use = m_cand;
           rescale = true;
         }
-        float sum = 0.f;
-        uint32_t pk[HC / 2];
+        l *= alpha;
+        uint32_t pk[16];
+        auto weigh = [&](int h) {
 #pragma unroll
-        for (int q = 0; q < HC / 16; ++q) {
-          const float lm = lg[q] - m_use;
-          const float2 c2 = make_float2(cg[q], cg[q]), l2 = make_float2(lm, lm);
-          float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+          for (int q = 0; q < 2; ++q) {
+            const float4 k4 = cc[2 * h + q];      // (read again: registers are what is short)
+            const float cq = fmaxf(k4.x * qs, 1e-37f), lm = k4.y - m_use;
+            const float2 c2 = make_float2(cq, cq), l2 = make_float2(lm, lm);
+            float2 a0 = make_float2(0.f, 0.f), a1 = a0;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float2 x = __ffma2_rn(make_float2(s[16 * q + 2 * k], s[16 * q + 2 * k + 1]), c2, l2);
-            if (edge) {                           // (a factor of 0 or not-a-number does not bring hidden keys back)
-              if (kv0 + 16 * q + 2 * k >= lim) x.x = -INFINITY;
-              if (kv0 + 16 * q + 2 * k + 1 >= lim) x.y = -INFINITY;
+            for (int k = 0; k < 8; ++k) {
+              const float2 x = __ffma2_rn(make_float2(s[16 * q + 2 * k], s[16 * q + 2 * k + 1]), c2, l2);
+              const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              if (k & 1) a1 = __fadd2_rn(a1, e);
+              else a0 = __fadd2_rn(a0, e);
+              pk[8 * q + k] = pack_half2(e.x, e.y);
             }
-            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            if (k & 1) a1 = __fadd2_rn(a1, e);
-            else a0 = __fadd2_rn(a0, e);
-            pk[8 * q + k] = pack_half2(e.x, e.y);
+            const float2 as = __fadd2_rn(a0, a1);
+            l = fmaf(as.x + as.y, k4.z, l);
           }
-          const float2 as = __fadd2_rn(a0, a1);
-          sum = fmaf(as.x + as.y, ig[q], sum);
+        };
+        // P of piece h: its columns, and those of the other half of the keys.
+        auto store = [&](int h) {
+          if constexpr (C::OVER) tmem_st_pair16<64>(t_p + 32 * h, pk);
+          else tmem_st_pair16<BN / 4>(t_p + 16 * h, pk);
+        };
+        weigh(NP - 1);
+        if constexpr (NP == 2) load(0);
+        if constexpr (!C::OVER) {                 // the next S may come
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[t]);
         }
-        l = fmaf(l, alpha, sum);
+        ++ns;
         if (np > 0) {                             // P and O are free once the last P V is done
           if (!mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc)) { ok = false; break; }
           tc_fence_after();
         }
-        if (j > it.j0 && __any_sync(0xffffffffu, rescale)) {
+        store(NP - 1);
+        if constexpr (NP == 2) {
+          weigh(0);
+          store(0);
+        }
+        if (j > jbeg && __any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+          for (int d = 0; d < OH; d += 16) {
+            uint32_t r[16];
+            tmem_ld_pair16<OH>(t_o + d, r);
 #pragma unroll
-          for (int d = 0; d < OH / OC; ++d) {
-            uint32_t r[OC];
-            if constexpr (OC == 16) tmem_ld_pair16<OH>(t_o, *reinterpret_cast<uint32_t(*)[16]>(r));
-            else tmem_ld_pair32<OH>(t_o + d * OC, *reinterpret_cast<uint32_t(*)[32]>(r));
-#pragma unroll
-            for (int k = 0; k < OC; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
-            if constexpr (OC == 16) tmem_st_pair16<OH>(t_o, *reinterpret_cast<uint32_t(*)[16]>(r));
-            else tmem_st_pair32<OH>(t_o + d * OC, *reinterpret_cast<uint32_t(*)[32]>(r));
+            for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+            tmem_st_pair16<OH>(t_o + d, r);
           }
         }
-        if constexpr (HC == 64) tmem_st_pair32<32>(t_p, *reinterpret_cast<uint32_t(*)[32]>(pk));
-        else tmem_st_pair16<16>(t_p, *reinterpret_cast<uint32_t(*)[16]>(pk));
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
@@ -575,39 +619,36 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       }
       if (!ok) break;
       // ---- the rows' results, or this piece of them
-      const bool any = it.j0 < it.j1;
+      const bool any = jbeg < jend;
       if (any) {
         if (!mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc)) { ok = false; break; }
         tc_fence_after();
       }
       const float lt = l + __shfl_xor_sync(0xffffffffu, l, 16);
       const float r1 = lt == 0.f ? 0.f : 1.0f / lt;
-      const long long xh = item / p.splits;
-      const long long pr = (xh * p.splits + it.piece) * C::MQ + t * 128 + row;
+      const long long pr = (long long)item * C::MQ + t * 128 + row;    // (item counts pieces)
       if (p.splits > 1 && in && c == 0) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(none ? -INFINITY : m_use, lt);
-      const long long oat = ((long long)(it.tok0 + i) * a.hq + hq) * a.dh;
-#pragma unroll
-      for (int d = 0; d < OH / OC; ++d) {
-        uint32_t r[OC];
+#pragma unroll 1
+      for (int d = 0; d < OH; d += 16) {
+        uint32_t r[16];
         if (any) {
-          if constexpr (OC == 16) tmem_ld_pair16<OH>(t_o, *reinterpret_cast<uint32_t(*)[16]>(r));
-          else tmem_ld_pair32<OH>(t_o + d * OC, *reinterpret_cast<uint32_t(*)[32]>(r));
+          tmem_ld_pair16<OH>(t_o + d, r);
         } else {
 #pragma unroll
-          for (int k = 0; k < OC; ++k) r[k] = 0u;
+          for (int k = 0; k < 16; ++k) r[k] = 0u;
         }
-        const int d0 = c * OH + d * OC;
+        const int d0 = c * OH + d;
         if (in) {
           if (p.splits > 1) {
             float4* o = reinterpret_cast<float4*>(a.part_o + pr * DHP + d0);
 #pragma unroll
-            for (int k = 0; k < OC / 4; ++k)
+            for (int k = 0; k < 4; ++k)
               o[k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]), __uint_as_float(r[4 * k + 2]),
                                  __uint_as_float(r[4 * k + 3]));
-          } else if (a.o_vec8 && d0 + OC <= a.dh) {
+          } else if (a.o_vec8 && d0 + 16 <= a.dh) {
             uint4* o = reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + oat + d0);
 #pragma unroll
-            for (int k = 0; k < OC / 8; ++k) {
+            for (int k = 0; k < 2; ++k) {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
@@ -616,7 +657,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
             }
           } else {
 #pragma unroll
-            for (int k = 0; k < OC; k += 2)
+            for (int k = 0; k < 16; k += 2)
               if (d0 + k < a.dh) store_out(a, oat, d0 + k, __uint_as_float(r[k]) * r1, __uint_as_float(r[k + 1]) * r1);
           }
         }
@@ -624,12 +665,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       }
       tc_fence_before();
     }
-  }
-  __syncthreads();
-  if (threadIdx.x == 0 && waitctl_aborted(wc)) record_error(status, -7, kKernelKvPrompt, 1);
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    block_end();
   }
 }
 
