@@ -198,9 +198,9 @@ struct KvAttnPlan {
   int dhp;
   bool prompt;                   // kv_prompt_kernel; else kv_decode_kernel
   int M, workers;                // decode: rows of a tile, warps
-  int tiles, splits;             // prompt: row tiles, pieces along the keys
+  int tiles, blocks;             // prompt: row tiles, stretches
   long long pieces;              // row tiles that the workspace holds
-  size_t off_o, total;
+  size_t off_plan, off_o, total;
 };
 
 int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAttnPlan* p) {
@@ -253,21 +253,15 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
   // bound by HBM; beyond, tcgen05's 128-row tiles.
   p->prompt = rows > 32;
   if (p->prompt) {
-    const int mq = p->dhp == 256 ? 128 : 256, bn = p->dhp == 256 ? 64 : 128;
+    const int mq = p->dhp == 256 ? 128 : 256;
     p->M = mq;
     p->workers = 0;
     a.row_tiles = a.min_units = a.whole = a.log2_unit = 0;
     p->tiles = (int)((long long)d->tokens * a.group / mq) + (d->requests < d->tokens ? d->requests : d->tokens);
-    const long long items = (long long)p->tiles * cache->num_heads;
-    // Few items: as many pieces along the keys as keep every SM busy, of at
-    // least four key tiles each where the table is full.
-    const long long keys = (long long)d->table_width * cache->page_size;
-    const long long most = keys / (4 * bn) > 1 ? keys / (4 * bn) : 1;
-    p->splits = (int)(items >= dev.sms ? 1 : dev.sms / items < most ? dev.sms / items : most);
-    if (items * p->splits > 0x7fffffffLL) return fail(B200L_ERR_BAD_SHAPE, "too many row tiles");
-    p->pieces = p->splits > 1 ? items * p->splits : 0;
+    p->blocks = dev.sms;
+    p->pieces = 2ll * p->blocks;
   } else {
-    p->tiles = p->splits = 0;
+    p->tiles = p->blocks = 0;
     p->M = rows <= 8 ? 8 : rows <= 16 || p->dhp == 256 ? 16 : 32;
     a.row_tiles = rows > p->M ? (rows + p->M - 1) / p->M : 1;
     const int tk = p->dhp == 256 ? 16 : p->dhp == 128 ? 32 : 64;
@@ -284,7 +278,8 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
     p->workers = 4 * (int)(blocks < full ? blocks : full);
     p->pieces = 2ll * p->workers;
   }
-  p->off_o = 1024;
+  p->off_plan = 1024;
+  p->off_o = p->prompt ? align_up(p->off_plan + ((size_t)p->tiles + p->blocks + 1) * 16 + ((size_t)p->tiles + 1) * 4, 1024) : 1024;
   p->total = align_up(p->off_o + (size_t)p->pieces * p->M * (p->dhp + 2) * 4, 1024);
   a.part_o = nullptr;
   a.part_ml = nullptr;
@@ -320,20 +315,19 @@ int kv_prompt_t(const KvAttnPlan& p, uint8_t* ws, cudaStream_t st) {
   auto kern = kv_prompt_kernel<DHP, KIND>;
   int rc = ensure_smem((const void*)kern, C::SMEM);
   if (rc) return rc;
-  DevInfo dev;
-  if ((rc = device_info(&dev))) return rc;
   KvPromptArgs pa;
   pa.a = p.a;
   pa.tiles = p.tiles;
-  pa.splits = p.splits;
-  pa.min_rows = 1;
-  const long long items = (long long)p.tiles * p.a.c.heads * p.splits;
-  const int grid = (int)(items < dev.sms ? items : dev.sms);
-  cudaError_t e = launch_pdl(kern, dim3(grid), dim3(C::THREADS), C::SMEM, st, pa, reinterpret_cast<DevStatus*>(ws));
+  pa.blocks = p.blocks;
+  pa.info = reinterpret_cast<int4*>(ws + p.off_plan);
+  pa.starts = pa.info + p.tiles;
+  pa.cum = reinterpret_cast<int*>(pa.starts + p.blocks + 1);
+  cudaError_t e = launch_pdl(kv_prompt_plan_kernel<DHP>, dim3(1), dim3(1024), 0, st, pa);
+  if (e != cudaSuccess) return cuda_fail(e, "kv_prompt_plan_kernel");
+  e = launch_pdl(kern, dim3(p.blocks), dim3(C::THREADS), C::SMEM, st, pa, reinterpret_cast<DevStatus*>(ws));
   if (e != cudaSuccess) return cuda_fail(e, "kv_prompt_kernel");
   if ((rc = check_launch("kv_prompt_kernel"))) return rc;
-  if (p.splits == 1) return B200L_OK;
-  e = launch_pdl(kv_prompt_join_kernel<DHP>, dim3(p.tiles * p.a.c.heads, 8), dim3(256), 0, st, pa);
+  e = launch_pdl(kv_prompt_join_kernel<DHP>, dim3(p.blocks, C::MQ / 8), dim3(256), 0, st, pa);
   if (e != cudaSuccess) return cuda_fail(e, "kv_prompt_join_kernel");
   return check_launch("kv_prompt_join_kernel");
 }

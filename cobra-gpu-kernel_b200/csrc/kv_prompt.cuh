@@ -3,8 +3,12 @@
 //
 // Same definition as kv_decode.cuh. A work item is (request, key head, 256 rows
 // = two tiles of 128 that share every K / V tile; 128 rows at dhp 256), a row
-// being one query head of one new token; items of few requests are cut along
-// the keys as well, and kv_prompt_join_kernel adds the pieces in order.
+// being one query head of one new token. The key tiles of all items in a row are
+// cut evenly over the SMs, as kv_decode.cuh cuts them over warps: a small kernel
+// sums them up first, a block works off its stretch, and of an item that is cut
+// each piece leaves (max, sum, accumulator), which kv_prompt_join_kernel adds in
+// order. An item counts for kItemCost key tiles more than it has, for that is what
+// its queries, its results and the pipeline between two items take.
 //
 // tcgen05 multiplies fp16, so codes become fp16 (exactly) on their way: bulk
 // copies bring a tile's pages as they lie into shared memory, four warps turn
@@ -35,11 +39,15 @@
 
 namespace b200l {
 
+constexpr int kItemCost = 4;
+
 struct KvPromptArgs {
-  KvAttnArgs a;                  // part_o / part_ml: [items][splits][rows]([dhp])
+  KvAttnArgs a;                  // part_o / part_ml: [2 * blocks][rows]([dhp])
+  int* cum;                      // [tiles + 1] cost of the row tiles before each, of one head
+  int4* info;                    // [tiles] a row tile's request, its first new token, their number, its keys
+  int4* starts;                  // [blocks + 1] where each stretch begins: row tile, head, key tile
   int tiles;                     // row tiles of all requests, at most
-  int splits;                    // pieces along the keys
-  int min_rows;                  // requests with fewer rows are the decode kernel's
+  int blocks;                    // stretches
 };
 
 template <int DHP>
@@ -57,7 +65,7 @@ struct KvPromptCfg {
   static constexpr int GR = BN / 16;                        // 16-key groups of a tile
   static constexpr int CSLOTS = 8;                          // stages of their constants
   static constexpr int SM_CONST = CSLOTS * (GR + 1) * 16;
-  static constexpr int SMEM = NQ * Q_BYTES + 4 * KV_BYTES + ST8 * 2 * C_BYTES + SM_CONST + 48 * 8 + 1024;
+  static constexpr int SMEM = NQ * Q_BYTES + 4 * KV_BYTES + ST8 * 2 * C_BYTES + SM_CONST + 48 * 8 + 4 * 48 + 1024;
   static constexpr int SOFT = NQ * 8;                       // softmax warps
   static constexpr int THREADS = 256 + 32 * SOFT;
   static constexpr int S_COL = 0;                           // + 128 t
@@ -70,44 +78,163 @@ struct KvPromptCfg {
   __host__ __device__ static constexpr int p_col(int k) { return OVER ? 64 * (k >> 2) + 32 * ((k >> 1) & 1) + 8 * (k & 1) : 8 * k; }
 };
 
-// A work item: rows [row0, row0 + MQ) of request r for key head h, key tiles [j0, j1).
-struct KvItem {
-  int r, h, row0, rows, n, len, tok0, nqt, j0, j1, piece;
-};
-
+// Where request r's row tiles begin: at floor(cu_new[r] group / MQ) + min(r,
+// cu_new[r]) there is room for every request with new tokens; what is left over
+// stays empty.
 template <int DHP>
-__device__ __forceinline__ bool kv_item(const KvPromptArgs& p, int item, int lane, KvItem& it) {
+__device__ __forceinline__ int kv_first_tile(const KvAttnArgs& a, int r, int cu) {
+  return (int)((long long)cu * a.group / KvPromptCfg<DHP>::MQ) + min(r, cu);
+}
+
+// The cost of every row tile (of one key tile at least, so that a row without
+// keys is written too) and their exclusive sums. One block; a warp takes 32 requests at a
+// time, a lane each, and all lanes the tiles of one that has many.
+template <int DHP>
+__global__ void __launch_bounds__(1024) kv_prompt_plan_kernel(const __grid_constant__ KvPromptArgs p) {
+  pdl_wait_then_release();
   using C = KvPromptCfg<DHP>;
   const KvAttnArgs& a = p.a;
-  it.piece = item % p.splits;
-  const int xh = item / p.splits;
-  it.h = xh % a.c.heads;
-  const int x = p.tiles - 1 - xh / a.c.heads;     // the last rows see the most keys: first
-  // Request r's tiles begin at floor(cu_new[r] group / MQ) + min(r, cu_new[r]):
-  // room for every request with new tokens; what is left over is skipped.
-  int lo = 0, hi = a.requests;
-  auto base = [&](int r) { return (int)((long long)a.cu_new[r] * a.group / C::MQ) + min(r, a.cu_new[r]); };
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
-    const int k = __popc(__ballot_sync(0xffffffffu, at < hi && base(at) <= x));
-    hi = min(hi, lo + (k + 1) * step);
-    lo += k * step;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < p.tiles; i += 1024) p.cum[i] = 0;
+  __syncthreads();
+  for (int r0 = warp * 32; r0 < a.requests; r0 += 1024) {
+    const int r = min(r0 + lane, a.requests - 1);
+    const int cu = a.cu_new[r], n = r0 + lane < a.requests ? a.cu_new[r + 1] - cu : 0;
+    const int len = min(max(a.lens[r], 0), min(a.cu_pages[r + 1] - a.cu_pages[r], a.width) << a.c.log2_page);
+    const long long rows = (long long)n * a.group;
+    const int nt = rows > 0 ? (int)((rows + C::MQ - 1) / C::MQ) : 0, first = kv_first_tile<DHP>(a, r, cu);
+    auto put = [&](int i, int req, int f, int tt, int nn, int ll) {  // row tile i of a request
+      const long long last = min((long long)(i + 1) * C::MQ, (long long)nn * a.group) - 1;
+      const int end = a.causal ? min(ll, max(0, ll - nn + (int)(last / a.group) + 1)) : ll;
+      if (f + i >= p.tiles) return;               // (cu_new is no prefix sum)
+      p.cum[f + i] = max(1, (end + C::BN - 1) / C::BN) + kItemCost;
+      p.info[f + i] = make_int4(req, tt, nn, ll);
+    };
+    if (nt > 0 && nt <= 2)
+      for (int i = 0; i < nt; ++i) put(i, r, first, cu, n, len);
+    unsigned many = __ballot_sync(0xffffffffu, nt > 2);
+    while (many) {
+      const int src = __ffs(many) - 1;
+      many &= many - 1;
+      const int f = __shfl_sync(0xffffffffu, first, src), nn = __shfl_sync(0xffffffffu, n, src);
+      const int ll = __shfl_sync(0xffffffffu, len, src), cc = __shfl_sync(0xffffffffu, cu, src);
+      const int count = __shfl_sync(0xffffffffu, nt, src);
+      for (int i = lane; i < count; i += 32) put(i, r0 + src, f, cc, nn, ll);
+    }
   }
-  it.r = lo;
-  it.tok0 = a.cu_new[lo];
-  it.n = a.cu_new[lo + 1] - it.tok0;
-  it.rows = it.n * a.group;
-  it.row0 = (x - base(lo)) * C::MQ;
-  if (it.row0 < 0 || it.row0 >= it.rows || it.rows < p.min_rows) return false;
-  it.nqt = it.rows - it.row0 > 128 && C::NQ == 2 ? 2 : 1;
-  it.len = min(max(a.lens[lo], 0), min(a.cu_pages[lo + 1] - a.cu_pages[lo], a.width) << a.c.log2_page);
-  const int last = min(it.row0 + C::MQ, it.rows) - 1;
-  const int end = a.causal ? min(it.len, max(0, it.len - it.n + last / a.group + 1)) : it.len;
-  const int nt = (end + C::BN - 1) / C::BN;
-  it.j0 = (int)((long long)nt * it.piece / p.splits);
-  it.j1 = (int)((long long)nt * (it.piece + 1) / p.splits);
-  return true;
+  __syncthreads();
+  __shared__ int part[32];
+  const int per = (p.tiles + 1023) / 1024, i0 = min(p.tiles, tid * per), i1 = min(p.tiles, i0 + per);
+  int sum = 0;
+  for (int i = i0; i < i1; ++i) sum += p.cum[i];
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) part[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int v = part[lane], s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    part[lane] = s - v;
+    if (lane == 31) p.cum[p.tiles] = s;
+  }
+  __syncthreads();
+  int at = part[warp] + inc - sum;
+  for (int i = i0; i < i1; ++i) {
+    const int v = p.cum[i];
+    p.cum[i] = at;
+    at += v;
+  }
+  __syncthreads();
+  // Where the stretches begin. Cost u of all lies in the item that it falls into, at
+  // the key tile past what the item itself costs; at its first one within that.
+  const long long all = (long long)a.c.heads * p.cum[p.tiles], mean = (all + p.blocks - 1) / p.blocks;
+  const long long c = mean < kItemCost + 2 ? kItemCost + 2 : mean;
+  for (int b = tid; b <= p.blocks; b += 1024) {
+    const long long u = b * c;
+    int4 s = make_int4(p.tiles, 0, 0, 0);
+    if (u < all) {
+      s.x = find_owner(p.cum, p.tiles, (int)(u / a.c.heads));
+      const int c0 = p.cum[s.x], w = p.cum[s.x + 1] - c0;
+      const long long off = u - (long long)c0 * a.c.heads;
+      s.y = (int)(off / w);
+      s.z = max(0, (int)(off - (long long)s.y * w) - kItemCost);
+    }
+    p.starts[b] = s;
+  }
 }
+
+// A piece of work: rows [row0, row0 + MQ) of a request for key head h, key tiles
+// [j0, j1). The loading warp finds them and leaves them in a ring for the others.
+struct KvItem {
+  int done;                      // nothing more to do
+  int j0, j1, len;
+  int nqt, row0, rows, n;
+  int tok0, h, slot;             // slot < 0: the whole item; else where the piece's results go
+  int pad;
+};
+static_assert(sizeof(KvItem) == 48, "four of them in 192 bytes");
+
+// The items of a stretch, one after another.
+template <int DHP>
+struct KvWalk {
+  int x, h, xe, he, je, nt, r;
+  KvItem it;
+  __device__ __forceinline__ void open(const KvPromptArgs& p) {
+    const int c0 = p.cum[x], c1 = p.cum[x + 1];
+    const int4 i = p.info[x];
+    nt = c1 - c0 - kItemCost;
+    r = i.x;
+    it.tok0 = i.y;
+    it.n = i.z;
+    it.len = i.w;
+    it.rows = i.z * p.a.group;
+    it.row0 = (x - kv_first_tile<DHP>(p.a, i.x, i.y)) * KvPromptCfg<DHP>::MQ;
+    it.nqt = it.rows - it.row0 > 128 && KvPromptCfg<DHP>::NQ == 2 ? 2 : 1;
+  }
+  // Slot 2b holds a piece that an earlier block began, 2b + 1 one that a later block goes on with.
+  __device__ __forceinline__ void cut(int b) {
+    const bool at_end = x == xe && h == he;
+    it.j1 = at_end ? je : nt;
+    it.h = h;
+    it.done = it.j0 >= it.j1;                     // (at the end, or both ends in what one item itself costs)
+    it.slot = it.j0 == 0 && it.j1 == nt ? -1 : 2 * b + (it.j0 == 0 ? 1 : 0);
+  }
+  __device__ __forceinline__ void begin(const KvPromptArgs& p, int b) {
+    const int4 s = p.starts[b], e = p.starts[b + 1];
+    x = s.x;
+    h = s.y;
+    it.j0 = s.z;
+    xe = e.x;
+    he = e.y;
+    je = e.z;
+    it.done = x >= p.tiles;
+    if (it.done) return;
+    open(p);
+    cut(b);
+  }
+  __device__ __forceinline__ void next(const KvPromptArgs& p, int b, int lane) {
+    it.done = x == xe && h == he;
+    if (it.done) return;
+    it.j0 = 0;
+    if (++h == p.a.c.heads) {
+      h = 0;
+      const int after = p.cum[x + 1];
+      it.done = after >= p.cum[p.tiles];          // that was the last one
+      if (it.done) return;
+      if (p.cum[++x + 1] == after) x = warp_find_owner(p.cum, p.tiles, after, lane);   // (empty ones)
+      open(p);
+    }
+    cut(b);
+  }
+};
 
 // Shared-memory descriptor of an MN-major B operand: K rows of ROWB bytes, 8 of
 // them a swizzle atom, atoms SBO = 8 ROWB apart along K and LBO along N.
@@ -125,10 +252,13 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 // The barrier that every warp ends on. Each kind of warp has its own, and never
 // meets the others' code again, so that its register count is its own too.
-__device__ __forceinline__ void block_end() { asm volatile("bar.sync 0;" ::: "memory"); }
+__device__ __forceinline__ void block_end() {
+  __syncwarp();
+  asm volatile("bar.sync 0;" ::: "memory");
+}
 
 template <int DHP, int KIND>
-__global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel(KvPromptArgs p, DevStatus* status) {
+__global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel(const __grid_constant__ KvPromptArgs p, DevStatus* status) {
   using C = KvPromptCfg<DHP>;
   constexpr int BN = C::BN, GR = C::GR, NP = BN / 64;   // pieces of 32 keys a thread
   const KvAttnArgs& a = p.a;
@@ -140,7 +270,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
   uint8_t* sV = sK + 2 * C::KV_BYTES;
   uint8_t* c8K = sV + 2 * C::KV_BYTES;
   uint8_t* c8V = c8K + C::ST8 * C::C_BYTES;
-  float4* consts = reinterpret_cast<float4*>(c8V + C::ST8 * C::C_BYTES);   // [CSLOTS][GR + 1]; the last: .x whole, .y poisoned
+  float4* consts = reinterpret_cast<float4*>(c8V + C::ST8 * C::C_BYTES);   // [CSLOTS][GR + 1]; the last: .x = plain
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(consts) + C::SM_CONST);
   uint64_t* q_full = bars;          // [2]
   uint64_t* q_empty = bars + 2;     // [2]
@@ -159,7 +289,10 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
   uint64_t* c_full = bars + 28;     // [CSLOTS]
   uint64_t* mma_done = bars + 36;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 37);
-  WaitCtl* wc = reinterpret_cast<WaitCtl*>(bars + 38);
+  WaitCtl* wc = reinterpret_cast<WaitCtl*>(bars + 38);   // 38, 39
+  uint64_t* i_full = bars + 40;     // [4]
+  uint64_t* i_free = bars + 44;     // [4]
+  KvItem* ring = reinterpret_cast<KvItem*>(bars + 48);   // [4]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -180,6 +313,10 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       mbar_init(&pv_done[i], 1);
     }
     for (int i = 0; i < C::CSLOTS; ++i) mbar_init(&c_full[i], 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&i_full[i], 1);
+      mbar_init(&i_free[i], 1 + C::NQ + 4 + C::SOFT);
+    }
     mbar_init(mma_done, 1 + C::NQ);
     waitctl_init(wc, status);
     fence_barrier_init();
@@ -191,27 +328,33 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int items = p.tiles * a.c.heads * p.splits;
   const int P = a.c.page, lp = a.c.log2_page, PB = P < BN ? P : BN;
 
   if (warp < 4) {
     if (warp == 0) {  // ================= pages and scales
       int g = 0, gk = 0, gv = 0;                  // tiles; K and V copies begun
       bool ok = true;
-      KvItem it;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        if (!kv_item<DHP>(p, item, lane, it)) continue;
-        const int* row = a.table + it.r * a.table_stride;
+      KvWalk<DHP> walk;
+      walk.begin(p, blockIdx.x);
+      for (int k = 0; ok; ++k, walk.next(p, blockIdx.x, lane)) {
+        if (!mbar_wait_warp(&i_free[k & 3], ((k >> 2) & 1) ^ 1, wc)) break;
+        if (lane == 0) {
+          ring[k & 3] = walk.it;
+          mbar_arrive(&i_full[k & 3]);
+        }
+        if (walk.it.done) break;
+        const int* row = a.table + walk.r * a.table_stride;
+        const int j0 = walk.it.j0, j1 = walk.it.j1, len = walk.it.len, head = walk.it.h;
         auto entry_at = [&](int j) {              // page of this lane's part of key tile j
           const int k = j * BN + lane * PB;
-          return (lane * PB < BN && k < it.len && (k >> lp) < a.width) ? row[k >> lp] : -1;
+          return (lane * PB < BN && k < len && (k >> lp) < a.width) ? row[k >> lp] : -1;
         };
-        int next = it.j0 < it.j1 ? entry_at(it.j0) : -1;
-        for (int j = it.j0; j < it.j1; ++j, ++g) {
+        int next = j0 < j1 ? entry_at(j0) : -1;
+        for (int j = j0; j < j1; ++j, ++g) {
           const int s8 = g % C::ST8, cs = g % C::CSLOTS, id = next;
-          if (j + 1 < it.j1) next = entry_at(j + 1);
+          if (j + 1 < j1) next = entry_at(j + 1);
           const bool there = id >= 0 && id < a.c.num_pages;
-          const long long ph = there ? (long long)id * a.c.heads + it.h : 0;
+          const long long ph = there ? (long long)id * a.c.heads + head : 0;
           const float sk = there ? a.c.k_scale[ph] : 0.f, sv = there ? a.c.v_scale[ph] : 0.f;
           const long long src = ((ph << lp) + ((j * BN + lane * PB) & (P - 1))) * DHP;
           const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, there));
@@ -224,8 +367,9 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
           bool poison = false;
           // The constants of this lane's keys, 16 at a time.
           if (lane * PB < BN) {
-            // w: 0 no such page, 1 a page, 2 one whose scales are no numbers: its visible
-            // scores become not-a-number, its constants are finite.
+            // w: 0 no such page, 1 a page, 2 one whose scales are no numbers: its keys
+            // become not-a-number, and their visible scores with them; its constants are
+            // finite.
             const bool fine = sk - sk == 0.f && sv - sv == 0.f;
             const float svc = fmaxf(sv, 7.8886090522101181e-31f);      // 2^-100 for a page of zeros
             float4 c;
@@ -236,11 +380,10 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
             poison = there && !fine;
             for (int i = 0; i < PB / 16; ++i) consts[cs * (GR + 1) + lane * (PB / 16) + i] = c;
           }
-          const int want = min(BN / PB, (it.len - j * BN + PB - 1) / PB);
+          const int want = min(BN / PB, (len - j * BN + PB - 1) / PB);
           poison = __any_sync(0xffffffffu, poison);
           if (lane == 0)
-            *reinterpret_cast<float2*>(&consts[cs * (GR + 1) + GR]) =
-                make_float2((int)boxes >= want && (j + 1) * BN <= it.len ? 1.f : 0.f, poison ? 1.f : 0.f);
+            consts[cs * (GR + 1) + GR].x = (int)boxes >= want && (j + 1) * BN <= len && !poison ? 1.f : 0.f;
           __syncwarp();
           if (lane == 0) mbar_arrive(&c_full[cs]);
           if (!mbar_wait_warp(&v8_free[s8], parity, wc)) { ok = false; break; }
@@ -261,16 +404,22 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       const uint64_t dk0 = sdesc_kmajor(smem_u32(sK), C::ROWB);
       int g = 0, ns[2] = {0, 0}, qi[2] = {0, 0};
       bool ok = true;
-      KvItem it;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        if (!kv_item<DHP>(p, item, lane, it) || it.j0 >= it.j1) continue;
+      for (int k = 0; ok; ++k) {
+        if (!mbar_wait_warp(&i_full[k & 3], (k >> 2) & 1, wc)) break;
+        // (shuffled, the values are known to be the same for all lanes: what is
+        // computed of them stays in uniform registers, as the products want it)
+        const int more = __shfl_sync(0xffffffffu, ring[k & 3].done ? 0 : 1, 0);
+        if (!more) break;
+        const int j0 = __shfl_sync(0xffffffffu, ring[k & 3].j0, 0), j1 = __shfl_sync(0xffffffffu, ring[k & 3].j1, 0);
+        const int nqt = __shfl_sync(0xffffffffu, ring[k & 3].nqt, 0);
         if (lane == 0) {
-          for (int t = 0; t < it.nqt && ok; ++t) ok = mbar_wait(&q_full[t], qi[t]++ & 1, wc);
-          for (int j = it.j0; j < it.j1 && ok; ++j, ++g) {
+          mbar_arrive(&i_free[k & 3]);
+          for (int t = 0; t < nqt && ok; ++t) ok = mbar_wait(&q_full[t], qi[t]++ & 1, wc);
+          for (int j = j0; j < j1 && ok; ++j, ++g) {
             const int st = g & 1;
             if (!mbar_wait(&k_full[st], (g >> 1) & 1, wc)) { ok = false; break; }
             const uint64_t dk = dk0 + (uint64_t)((st * C::KV_BYTES) >> 4);
-            for (int t = 0; t < it.nqt; ++t) {
+            for (int t = 0; t < nqt; ++t) {
               // S_t's columns are free once the softmax has read them; where P
               // takes their place, once P V has read that.
               if (ns[t] > 0 && !mbar_wait(C::OVER ? &pv_done[t] : &s_free[t], (ns[t] - 1) & 1, wc)) { ok = false; break; }
@@ -290,7 +439,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
             if (ok) umma_commit(&k_empty[st]);
           }
           if (ok)
-            for (int t = 0; t < it.nqt; ++t) umma_commit(&q_empty[t]);
+            for (int t = 0; t < nqt; ++t) umma_commit(&q_empty[t]);
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
@@ -309,20 +458,26 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       const uint32_t d_o = tmem_base + C::O_COL + t * C::O_STEP;
       int g = 0, np = 0;
       bool ok = true;
-      KvItem it;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        if (!kv_item<DHP>(p, item, lane, it) || it.j0 >= it.j1) continue;
+      for (int k = 0; ok; ++k) {
+        if (!mbar_wait_warp(&i_full[k & 3], (k >> 2) & 1, wc)) break;
+        // (shuffled, the values are known to be the same for all lanes: what is
+        // computed of them stays in uniform registers, as the products want it)
+        const int more = __shfl_sync(0xffffffffu, ring[k & 3].done ? 0 : 1, 0);
+        if (!more) break;
+        const int j0 = __shfl_sync(0xffffffffu, ring[k & 3].j0, 0), j1 = __shfl_sync(0xffffffffu, ring[k & 3].j1, 0);
+        const int nqt = __shfl_sync(0xffffffffu, ring[k & 3].nqt, 0);
         if (lane == 0) {
-          for (int j = it.j0; j < it.j1 && ok; ++j, ++g) {
+          mbar_arrive(&i_free[k & 3]);
+          for (int j = j0; j < j1 && ok; ++j, ++g) {
             const int st = g & 1;
             if (!mbar_wait(&v_full[st], (g >> 1) & 1, wc)) { ok = false; break; }
-            if (t >= it.nqt) {                    // no second tile: the stage is released as it comes
+            if (t >= nqt) {                    // no second tile: the stage is released as it comes
               umma_commit(&v_empty[st]);
               continue;
             }
             if (!mbar_wait(&p_full[t], np & 1, wc)) { ok = false; break; }
             const uint64_t dv = dv0 + (uint64_t)((st * C::KV_BYTES) >> 4);
-            const uint32_t acc0 = j > it.j0 ? 1u : 0u;
+            const uint32_t acc0 = j > j0 ? 1u : 0u;
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < BN / 16; ++k)
@@ -350,14 +505,17 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
     constexpr int UPH = C::ROWB / 32;             // ... of a swizzled fp16 row
     int g = 0;
     bool ok = true;
-    KvItem it;
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      if (!kv_item<DHP>(p, item, lane, it)) continue;
-      for (int j = it.j0; j < it.j1 && ok; ++j, ++g) {
+    for (int k = 0; ok; ++k) {
+      if (!mbar_wait_warp(&i_full[k & 3], (k >> 2) & 1, wc)) break;
+      if (ring[k & 3].done) break;
+      const int j0 = ring[k & 3].j0, j1 = ring[k & 3].j1, len = ring[k & 3].len;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&i_free[k & 3]);
+      for (int j = j0; j < j1 && ok; ++j, ++g) {
         const int s8 = g % C::ST8, cs = g % C::CSLOTS, st = g & 1;
         if (!mbar_wait_warp(&c_full[cs], (g / C::CSLOTS) & 1, wc)) { ok = false; break; }
         const float4* cc = consts + cs * (GR + 1);
-        const bool whole = cc[GR].x != 0.f;
+        const bool plain = cc[GR].x != 0.f;       // every key there, and a number
 #pragma unroll 1
         for (int which = 0; which < 2; ++which) {
           uint64_t* full8 = which ? &v8_full[s8] : &k8_full[s8];
@@ -379,13 +537,18 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
               const int unit = (u0 + i) * 128 + tid, row = unit / UPR, c16 = unit % UPR;
-              // What lies past the keys, or in a page that is not there, is no number.
-              if (!whole && (j * BN + row >= it.len || cc[row >> 4].w == 0.f)) w[i] = make_uint4(0, 0, 0, 0);
+              // What lies past the keys, or in a page that is not there, is no code.
+              const float page = plain ? 1.f : cc[row >> 4].w;
+              if (!plain && (j * BN + row >= len || page == 0.f)) w[i] = make_uint4(0, 0, 0, 0);
               uint32_t h[8];
               codes4_to_half<KIND>(w[i].x, h[0], h[1]);
               codes4_to_half<KIND>(w[i].y, h[2], h[3]);
               codes4_to_half<KIND>(w[i].z, h[4], h[5]);
               codes4_to_half<KIND>(w[i].w, h[6], h[7]);
+              if (page == 2.f && which == 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[e] = 0x7e007e00u;
+              }
               const int hb = c16 / UPH, ch = 2 * (c16 % UPH), odd = hb & 1;
               const uint32_t base = dst + hb * BN * C::ROWB;
               // (neighbouring halves write their odd pieces first: no bank conflicts)
@@ -421,11 +584,14 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
                    e = (long long)a.tokens * a.hq * a.dh;
          i < e; i += (long long)gridDim.x * C::SOFT * 32)
       static_cast<unsigned short*>(a.out)[i] = 0;
-    KvItem it;
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      if (!kv_item<DHP>(p, item, lane, it)) continue;
+    for (int k = 0; ok; ++k) {
+      if (!mbar_wait_warp(&i_full[k & 3], (k >> 2) & 1, wc)) break;
+      const volatile KvItem& it = ring[k & 3];    // (read again after the tiles: registers are what is short)
+      if (it.done) break;
       if (t >= it.nqt) {
         g += it.j1 - it.j0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&i_free[k & 3]);
         continue;
       }
       const int gr = it.row0 + t * 128 + row, i = gr / a.group, hq = it.h * a.group + gr - i * a.group;
@@ -433,16 +599,15 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       const int lim = !in ? 0 : a.causal ? min(it.len, it.len - it.n + i + 1) : it.len;
       const int first = (it.row0 + t * 128) / a.group;              // the tile's first token sees least
       const int lim_min = a.causal ? min(it.len, it.len - it.n + first + 1) : it.len;
-      const long long oat = ((long long)(it.tok0 + i) * a.hq + hq) * a.dh;
       const int jbeg = it.j0, jend = it.j1;
       float qs = a.scale_log2, m_use = 0.f, l = 0.f;
       bool none = true;                           // no visible key so far
-      if (jbeg < jend) {  // ---- the row of Q as fp16, scaled by a power of two if it comes as bf16
+      {  // ---- the row of Q as fp16, scaled by a power of two if it comes as bf16
         const long long at = (long long)(it.tok0 + i) * a.q_st + (long long)hq * a.q_sh;
         const uint4* q8 = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + at);
         const unsigned short* q1 = static_cast<const unsigned short*>(a.q) + at;
-        auto load8 = [&](int d) {                 // dims [d, d + 8)
-          if (in && a.q_vec8 && d + 8 <= a.dh) return q8[d / 8];
+        const bool vec = a.q_vec8 && DHP == a.dh;  // (uniform)
+        auto slow8 = [&](int d) {                 // dims [d, d + 8), one by one
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -452,43 +617,55 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
           }
           return make_uint4(w[0], w[1], w[2], w[3]);
         };
+        const uint32_t dst = smem_u32(sQ + t * C::Q_BYTES);
+        auto put8 = [&](int d, uint4 u) {
+          const int chunk = d / 8;
+          st_shared_v4(dst + (chunk / (C::ROWB / 16)) * 128 * C::ROWB + swz_offset(row, chunk % (C::ROWB / 16), C::ROWB), u.x,
+                       u.y, u.z, u.w);
+        };
+        constexpr int QC = OH / 8 < 4 ? OH / 8 : 4;   // pieces of 8 dims under way at once
         float mul = 1.f;
         if (a.type == kElemBF16) {
-          float big = 0.f;
-#pragma unroll 4
-          for (int d = 0; d < OH; d += 8) {
-            const uint4 u = load8(c * OH + d);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          // The largest of the row: as whole numbers, values without their sign are in order.
+          uint32_t big = 0;
+#pragma unroll 1
+          for (int d = 0; d < OH; d += 8 * QC) {
+            uint4 u[QC];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
-              big = fmax3f(big, fabsf(f.x), fabsf(f.y));
-            }
+            for (int k = 0; k < QC; ++k)
+              u[k] = vec ? (in ? q8[(c * OH + d) / 8 + k] : make_uint4(0, 0, 0, 0)) : slow8(c * OH + d + 8 * k);
+#pragma unroll
+            for (int k = 0; k < QC; ++k)
+              big = __vmaxu2(big, __vmaxu2(__vmaxu2(u[k].x & 0x7fff7fffu, u[k].y & 0x7fff7fffu),
+                                           __vmaxu2(u[k].z & 0x7fff7fffu, u[k].w & 0x7fff7fffu)));
           }
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
-          if (big > 0.f && big < INFINITY) {
-            const int ex = min(max(((__float_as_int(big) >> 23) & 255) - 127, -120), 120);
+          big = max(big & 0xffffu, big >> 16);
+          big = max(big, __shfl_xor_sync(0xffffffffu, big, 16));
+          if (big != 0 && big < 0x7f80u) {
+            const int ex = min(max((int)(big >> 7) - 127, -120), 120);
             mul = __int_as_float((127 - ex) << 23);
             qs *= __int_as_float((127 + ex) << 23);
           }
         }
         if (!mbar_wait_warp(&q_empty[t], (qi & 1) ^ 1, wc)) { ok = false; break; }
         ++qi;
-        const uint32_t dst = smem_u32(sQ + t * C::Q_BYTES);
-#pragma unroll 4
-        for (int d = 0; d < OH; d += 8) {
-          const uint4 u = load8(c * OH + d);
-          uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll 1
+        for (int d = 0; d < OH; d += 8 * QC) {
+          uint4 u[QC];
+#pragma unroll
+          for (int k = 0; k < QC; ++k)
+            u[k] = vec ? (in ? q8[(c * OH + d) / 8 + k] : make_uint4(0, 0, 0, 0)) : slow8(c * OH + d + 8 * k);
           if (a.type == kElemBF16) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
-              w[k] = pack_half2(f.x * mul, f.y * mul);
+            for (int k = 0; k < QC; ++k) {
+              uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack_half2(__uint_as_float(w[e] << 16) * mul, __uint_as_float(w[e] & 0xffff0000u) * mul);
+              u[k] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
-          const int chunk = (c * OH + d) / 8;
-          st_shared_v4(dst + (chunk / (C::ROWB / 16)) * 128 * C::ROWB + swz_offset(row, chunk % (C::ROWB / 16), C::ROWB), w[0],
-                       w[1], w[2], w[3]);
+#pragma unroll
+          for (int k = 0; k < QC; ++k) put8(c * OH + d + 8 * k, u[k]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -504,7 +681,6 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
         // This thread's keys: 32 NP from BN/2 c on, in pieces of 32.
         const float4* cc = consts + cs * (GR + 1) + c * (GR / 2);
         const bool edge = (j + 1) * BN > lim_min; // (warp-uniform)
-        const bool poison = consts[cs * (GR + 1) + GR].y != 0.f;
         float s[32];
         auto load = [&](int h) {
           tmem_ld_pair32<BN / 2>(t_s + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(s));
@@ -513,15 +689,6 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               if (k >= left) s[k] = -INFINITY;
-          }
-          if (poison) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-              if (cc[2 * h + q].w == 2.f) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                  if (s[16 * q + k] != -INFINITY) s[16 * q + k] = __int_as_float(0x7fc00000);
-              }
           }
         };
         // (A factor is above 0, so that hidden keys stay hidden: -inf * 0 is no number.)
@@ -540,26 +707,6 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
           }
           return fmaxf(m[0], m[1]);
         };
-        load(0);
-        float hm = top(0);
-        if constexpr (NP == 2) {
-          load(1);
-          hm = fmaxf(hm, top(1));
-        }
-        const float m_cand = fmaxf(hm, __shfl_xor_sync(0xffffffffu, hm, 16));
-        float alpha = 1.f;
-        bool rescale = false;
-        if (none) {
-          if (m_cand > -INFINITY) {
-            none = false;
-            m_use = m_cand;
-          }
-        } else if (m_cand > m_use + 8.f) {
-          alpha = ex2_approx(m_use - m_cand);
-          m_use = m_cand;
-          rescale = true;
-        }
-        l *= alpha;
         uint32_t pk[16];
         auto weigh = [&](int h) {
 #pragma unroll
@@ -585,23 +732,47 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
           if constexpr (C::OVER) tmem_st_pair16<64>(t_p + 32 * h, pk);
           else tmem_st_pair16<BN / 4>(t_p + 16 * h, pk);
         };
-        weigh(NP - 1);
-        if constexpr (NP == 2) load(0);
-        if constexpr (!C::OVER) {                 // the next S may come
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[t]);
+        float hm = -INFINITY, alpha = 1.f;
+        bool rescale = false;
+        // The pieces' maxima, the last one's weights, the first one's: one loop, for the
+        // sake of the instruction caches, which four kinds of warps share.
+#pragma unroll 1
+        for (int pass = 0; pass < 2 * NP - 1; ++pass) {
+          const int h = NP == 2 ? pass & 1 : 0;
+          load(h);
+          if (pass < NP) hm = fmaxf(hm, top(h));
+          if (pass < NP - 1) continue;
+          if (pass == NP - 1) {
+            const float m_cand = fmaxf(hm, __shfl_xor_sync(0xffffffffu, hm, 16));
+            if (none) {
+              if (m_cand > -INFINITY) {
+                none = false;
+                m_use = m_cand;
+              }
+            } else if (m_cand > m_use + 8.f) {
+              alpha = ex2_approx(m_use - m_cand);
+              m_use = m_cand;
+              rescale = true;
+            }
+            l *= alpha;
+          }
+          if (pass == 2 * NP - 2) {
+            if constexpr (!C::OVER) {             // the next S may come
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_free[t]);
+            }
+          }
+          weigh(h);
+          if (pass == NP - 1 && np > 0) {         // P and O are free once the last P V is done
+            ok = mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          store(h);
         }
+        if (!ok) break;
         ++ns;
-        if (np > 0) {                             // P and O are free once the last P V is done
-          if (!mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc)) { ok = false; break; }
-          tc_fence_after();
-        }
-        store(NP - 1);
-        if constexpr (NP == 2) {
-          weigh(0);
-          store(0);
-        }
         if (j > jbeg && __any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
           for (int d = 0; d < OH; d += 16) {
@@ -619,27 +790,22 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
       }
       if (!ok) break;
       // ---- the rows' results, or this piece of them
-      const bool any = jbeg < jend;
-      if (any) {
-        if (!mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc)) { ok = false; break; }
-        tc_fence_after();
-      }
+      if (!mbar_wait_warp(&pv_done[t], (np - 1) & 1, wc)) { ok = false; break; }
+      tc_fence_after();
       const float lt = l + __shfl_xor_sync(0xffffffffu, l, 16);
       const float r1 = lt == 0.f ? 0.f : 1.0f / lt;
-      const long long pr = (long long)item * C::MQ + t * 128 + row;    // (item counts pieces)
-      if (p.splits > 1 && in && c == 0) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(none ? -INFINITY : m_use, lt);
+      const int slot = it.slot, gr2 = it.row0 + t * 128 + row, i2 = gr2 / a.group, tok = it.tok0 + i2;
+      const bool whole = slot < 0, mine = gr2 < it.rows && tok < a.tokens;
+      const long long oat = ((long long)tok * a.hq + it.h * a.group + gr2 - i2 * a.group) * a.dh;
+      const long long pr = (long long)slot * C::MQ + t * 128 + row;
+      if (!whole && mine && c == 0) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(none ? -INFINITY : m_use, lt);
 #pragma unroll 1
       for (int d = 0; d < OH; d += 16) {
         uint32_t r[16];
-        if (any) {
-          tmem_ld_pair16<OH>(t_o + d, r);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) r[k] = 0u;
-        }
+        tmem_ld_pair16<OH>(t_o + d, r);
         const int d0 = c * OH + d;
-        if (in) {
-          if (p.splits > 1) {
+        if (mine) {
+          if (!whole) {
             float4* o = reinterpret_cast<float4*>(a.part_o + pr * DHP + d0);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -664,28 +830,40 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
         __syncwarp();
       }
       tc_fence_before();
+      if (lane == 0) mbar_arrive(&i_free[k & 3]);
     }
     block_end();
   }
 }
 
-// Adds the pieces of each row in order; a warp per row, the rows of an item
-// spread over blocks.
+// Adds the pieces of every item that was cut, in order. blockIdx.x: the stretch
+// that the item begins in and goes on past; blockIdx.y: eight of its rows, a warp
+// each.
 template <int DHP>
-__global__ void __launch_bounds__(256) kv_prompt_join_kernel(KvPromptArgs p) {
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_constant__ KvPromptArgs p) {
   pdl_wait_then_release();
   using C = KvPromptCfg<DHP>;
   const KvAttnArgs& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  KvItem it;
-  const int item = blockIdx.x * p.splits;         // (its first piece)
-  if (!kv_item<DHP>(p, item, lane, it)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = blockIdx.x;
+  const int4 from = p.starts[w], to = p.starts[w + 1];
+  // The stretch's end cuts an item, and its beginning does not cut the same one.
+  if (to.x >= p.tiles || to.z == 0 || (from.x == to.x && from.y == to.y && from.z > 0)) return;
+  KvWalk<DHP> walk;
+  walk.x = to.x;
+  walk.open(p);
+  KvItem& it = walk.it;
+  it.h = to.y;
+  int pieces = 2;
+  for (int b = w + 2; b <= p.blocks; ++b, ++pieces) {
+    const int4 s = p.starts[b];
+    if (s.x != to.x || s.y != to.y) break;
+  }
+  auto slot = [&](int i) { return i == 0 ? 2 * w + 1 : 2 * (w + i); };
   for (int row = blockIdx.y * 8 + warp; row < C::MQ; row += gridDim.y * 8) {
     const int gr = it.row0 + row, i = gr / a.group;
     if (gr >= it.rows || it.tok0 + i >= a.tokens) break;
-    const long long at = (long long)item * C::MQ + row;              // + piece * MQ
     float top = -INFINITY;
-    for (int k = lane; k < p.splits; k += 32) top = fmaxf(top, a.part_ml[(at + (long long)k * C::MQ) * 2]);
+    for (int k = lane; k < pieces; k += 32) top = fmaxf(top, a.part_ml[((long long)slot(k) * C::MQ + row) * 2]);
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
     if (top == -INFINITY) top = 0.f;
@@ -694,8 +872,8 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(KvPromptArgs p) {
 #pragma unroll
     for (int d = 0; d < PER; ++d) acc[d] = 0.f;
 #pragma unroll 4
-    for (int k = 0; k < p.splits; ++k) {
-      const long long pr = at + (long long)k * C::MQ;
+    for (int k = 0; k < pieces; ++k) {
+      const long long pr = (long long)slot(k) * C::MQ + row;
       const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + pr * 2);
       const float f = ex2_approx(ml.x - top);
       l = fmaf(ml.y, f, l);
