@@ -21,7 +21,7 @@ EXPORTED = (
     "b200l_block_forward", "b200l_row_layernorm", "b200l_cast_f16",
     "b200l_kernel_workspace_bytes", "b200l_debug_arm", "b200l_noalloc_read_status",
     "b200l_convert",
-    "b200l_kv_plan", "b200l_kv_append", "b200l_kv_read",
+    "b200l_block_finish", "b200l_kv_plan", "b200l_kv_append", "b200l_kv_read",
     "b200l_kv_attention_workspace_bytes", "b200l_kv_attention",
 )
 
@@ -147,6 +147,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200l_layer_forward_noalloc": (c_int, [P, P, P, P]),
         "b200l_block_workspace_bytes": (c_size_t, [P]),
         "b200l_block_forward": (c_int, [P, P, P, P, c_size_t, P]),
+        "b200l_block_finish": (c_int, [P, P, P, P, c_size_t, P]),
         "b200l_row_layernorm": (c_int, [P, P, P, P, c_float, ctypes.c_int64, c_int32, P, P]),
         "b200l_cast_f16": (c_int, [P, P, ctypes.c_int64, P]),
         "b200l_kernel_workspace_bytes": (c_size_t, [P]),

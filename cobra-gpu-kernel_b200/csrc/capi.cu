@@ -627,8 +627,8 @@ int run_resid_gemm(const void* a, int K, const void* bmat, int d, const float* b
   }
 }
 
-int run_block(const b200l_block_desc* bd, const BlockPlan& bp, const DevInfo& dev, const float* x, float* y,
-              void* ws, cudaStream_t st) {
+// The block from ctx in the workspace on.
+int run_block_finish(const b200l_block_desc* bd, const BlockPlan& bp, const float* x, float* y, void* ws, cudaStream_t st) {
   const b200l_layer_desc* desc = &bd->layer;
   const Plan& p = bp.p;
   uint8_t* w = static_cast<uint8_t*>(ws);
@@ -636,8 +636,6 @@ int run_block(const b200l_block_desc* bd, const BlockPlan& bp, const DevInfo& de
   __half* h2 = reinterpret_cast<__half*>(w + bp.off_h2);
   __half* h1 = reinterpret_cast<__half*>(w + bp.off_h1);
   int rc;
-  if ((rc = run_qkv(desc, p, x, ws, st))) return rc;
-  if ((rc = run_attn(desc, p, dev, ws, st))) return rc;
   // x1 = x + (valid row ? ctx Wo^T + bo : 0)
   if ((rc = run_resid_gemm(w + p.off_ctx, p.d, desc->wo, p.d, desc->bo, x, x1, desc->valid_mask, 0, p.T, ws, st)))
     return rc;
@@ -654,6 +652,14 @@ int run_block(const b200l_block_desc* bd, const BlockPlan& bp, const DevInfo& de
   }
   // y = valid row ? x1 + h1 W2^T + b2 : 0
   return run_resid_gemm(h1, bp.f, bd->w2, p.d, bd->b2, x1, y, desc->valid_mask, 1, p.T, ws, st);
+}
+
+int run_block(const b200l_block_desc* bd, const BlockPlan& bp, const DevInfo& dev, const float* x, float* y,
+              void* ws, cudaStream_t st) {
+  int rc;
+  if ((rc = run_qkv(&bd->layer, bp.p, x, ws, st))) return rc;
+  if ((rc = run_attn(&bd->layer, bp.p, dev, ws, st))) return rc;
+  return run_block_finish(bd, bp, x, y, ws, st);
 }
 
 int check_xy(const void* x, const void* y, bool need_y) {
@@ -786,20 +792,35 @@ size_t b200l_block_workspace_bytes(const b200l_block_desc* desc) {
   return bp.total;
 }
 
+static int check_block(const b200l_block_desc* desc, const float* x, float* y, void* workspace, size_t ws_bytes,
+                       const char* entry, BlockPlan* bp, DevInfo* dev) {
+  int rc = make_block_plan(desc, bp);
+  if (rc) return rc;
+  if (bp->p.Hl != bp->p.H) return fail(B200L_ERR_BAD_SHAPE, "%s computes every head: local_heads must be 0", entry);
+  if (!desc->w1 || !desc->b1 || !desc->w2 || !desc->b2) return fail(B200L_ERR_NULL_POINTER, "FFN weight is NULL");
+  Plan p;
+  if ((rc = check_common(&desc->layer, workspace, ws_bytes, &p, dev))) return rc;
+  if (ws_bytes < bp->total)
+    return fail(B200L_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes < %zu needed", ws_bytes, bp->total);
+  return check_xy(x, y, true);
+}
+
 int b200l_block_forward(const b200l_block_desc* desc, const float* x, float* y, void* workspace, size_t ws_bytes,
                         void* stream) {
   BlockPlan bp;
-  int rc = make_block_plan(desc, &bp);
-  if (rc) return rc;
-  if (bp.p.Hl != bp.p.H) return fail(B200L_ERR_BAD_SHAPE, "b200l_block_forward computes every head: local_heads must be 0");
-  if (!desc->w1 || !desc->b1 || !desc->w2 || !desc->b2) return fail(B200L_ERR_NULL_POINTER, "FFN weight is NULL");
-  Plan p;
   DevInfo dev;
-  if ((rc = check_common(&desc->layer, workspace, ws_bytes, &p, &dev))) return rc;
-  if (ws_bytes < bp.total)
-    return fail(B200L_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes < %zu needed", ws_bytes, bp.total);
-  if ((rc = check_xy(x, y, true))) return rc;
+  int rc = check_block(desc, x, y, workspace, ws_bytes, "b200l_block_forward", &bp, &dev);
+  if (rc) return rc;
   return run_block(desc, bp, dev, x, y, workspace, static_cast<cudaStream_t>(stream));
+}
+
+int b200l_block_finish(const b200l_block_desc* desc, const float* x, float* y, void* workspace, size_t ws_bytes,
+                       void* stream) {
+  BlockPlan bp;
+  DevInfo dev;
+  int rc = check_block(desc, x, y, workspace, ws_bytes, "b200l_block_finish", &bp, &dev);
+  if (rc) return rc;
+  return run_block_finish(desc, bp, x, y, workspace, static_cast<cudaStream_t>(stream));
 }
 
 int b200l_row_layernorm(const float* x, float* y, const float* w, const float* b, float eps, int64_t rows,

@@ -381,3 +381,74 @@ def _attention(stream, index, c, desc) -> None:
         rc = L.b200l_kv_attention(c, desc, ws, size, stream)
     if rc:
         _lib.check(rc)
+
+
+# ---------------------------------------------------------------- between steps
+class KVPool:
+    """What a server keeps of its requests between steps: cached lengths, block
+    table and free pages, on the GPU. Row r of each is one place for a request;
+    a place is given up by a new length of 0.
+
+        plan = pool.plan(new_lens, max_tokens)
+        ...                                      # kv_append and kv_attention, layer by layer
+        pool.adopt(new_lens, plan)
+    """
+
+    def __init__(self, requests: int, pages_per_request: int, num_pages: int, *, page_size: int = 64, device="cuda") -> None:
+        if requests <= 0 or pages_per_request <= 0 or num_pages <= 0:
+            raise ValueError("requests, pages_per_request and num_pages must be positive")
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+        i32 = dict(dtype=torch.int32, device=device)
+        self.page_size = page_size
+        self.lens = torch.zeros(requests, **i32)
+        self.block_table = torch.full((requests, pages_per_request), -1, **i32)
+        self.free_pages = torch.arange(num_pages, **i32)
+        self.free_count = torch.full((1,), num_pages, **i32)
+
+    def plan(self, new_lens: torch.Tensor, max_tokens: int) -> KVPlan:
+        """``kv_plan`` from the pool's lengths to ``new_lens`` (int32 ``[requests]``)."""
+        return kv_plan(self.lens, new_lens, self.block_table, self.free_pages, self.free_count, page_size=self.page_size,
+                       max_tokens=max_tokens)
+
+    def adopt(self, new_lens: torch.Tensor, plan: KVPlan) -> None:
+        """Goes on from the lengths and free pages of a plan that missed no pages."""
+        self.lens.copy_(new_lens)
+        self.free_count.copy_(plan.info[:1])
+
+
+def attend_cached(lib_qkv, views, cache: KVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, plan: KVPlan,
+                  max_new: int, causal: bool) -> None:
+    """The attention of a cached layer step: ``lib_qkv()`` fills the q / k / v^T
+    regions of a workspace with the new tokens, ``views`` are (q, k, v, ctx) on it
+    (``workspace_views``); the new keys and values go to the cache, and ctx is
+    attention over it."""
+    q, k, v, ctx = views
+    lib_qkv()
+    kv_append(k, v, plan.slots, cache)
+    kv_attention(q, cache, block_table, seq_lens, plan, max_new=max_new, causal=causal, out=ctx)
+
+
+def workspace_views(ws: torch.Tensor, lay: dict, T: int, heads: int):
+    """q, k, v and ctx of one sequence of T tokens in a layer workspace (bytes from
+    its start; ``_lib.workspace_layout``), as ``[T, heads, head_dim]`` fp16."""
+    dh, dhp, sp = lay["dh"], lay["dhp"], lay["sp"]
+
+    def region(name: str, shape) -> torch.Tensor:
+        n = 2 * shape[0] * shape[1] * shape[2]
+        return ws[lay[name]:lay[name] + n].view(torch.float16).view(shape)
+
+    q, k = (region(n, (heads, T, dhp))[..., :dh].transpose(0, 1) for n in ("q", "k"))
+    v = region("vt", (heads, dhp, sp))[:, :dh, :T].permute(2, 0, 1)
+    return q, k, v, region("ctx", (T, heads, dh))
+
+
+def check_step(x: torch.Tensor, d: int, plan: KVPlan) -> None:
+    """x of a cached step: fp32 [tokens, d] on the GPU, at most the plan's tokens."""
+    if x.dim() != 2 or x.shape[-1] != d or x.shape[0] == 0:
+        raise ValueError(f"expected x of shape [tokens, {d}], got {tuple(x.shape)}")
+    if x.dtype != torch.float32:
+        raise TypeError(f"a cached step takes fp32 x, got {x.dtype}")
+    _cuda(x, "x")
+    if plan.slots.shape[0] < x.shape[0]:
+        raise ValueError(f"x has {x.shape[0]} tokens, the plan slots for {plan.slots.shape[0]}")

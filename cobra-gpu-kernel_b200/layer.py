@@ -31,7 +31,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _lib, kvcache
 
 GRAPH_MAX_INPUT_BYTES = 64 * 1024 * 1024   # reference gate, torch_transformer_benchmark.py:1077-1079
 _REDUCED = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}   # converted at the boundary
@@ -383,6 +383,36 @@ class B200TransformerLayer(nn.Module):
             y = out if out is not None else torch.empty_like(x)
             self._launch(x, y, desc)
             return y
+
+    def forward_cached(self, x: torch.Tensor, cache: kvcache.KVCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                       plan: kvcache.KVPlan, *, max_new: int) -> torch.Tensor:
+        """y of new tokens that attend to their requests' cached ones (and, first
+        written there, to themselves): LN1 + QKV, ``kv_append``, ``kv_attention``,
+        out-projection + residual + LN2.
+
+        ``x`` is fp32 [tokens, d], the new tokens of all requests one after
+        another as ``plan`` (``kv_plan``) has them; ``seq_lens`` the cached lengths
+        after the step; ``max_new`` the most new tokens of a request. With
+        ``causal`` a token sees what comes before it and itself, else all that is
+        cached. Returns a new tensor. Rows past the plan's tokens see no keys."""
+        d, H = self.attention.d_model, self.attention.num_heads
+        kvcache.check_step(x, d, plan)
+        x = x.contiguous()
+        T, dev, L = x.shape[0], x.device, _lib.lib()
+        with torch.cuda.device(dev):
+            pk = self._ensure_pack(dev)
+            desc = self._desc(1, T, pk)
+            self._ensure_workspace(desc, dev, stepwise=True)
+            lay = _lib.workspace_layout(1, T, d, H)
+            st = torch.cuda.current_stream(dev).cuda_stream
+            kvcache.attend_cached(
+                lambda: _lib.check(L.b200l_qkv_ln_gemm(ctypes.byref(desc), x.data_ptr(), self.workspace_ptr, self._ws_bytes, st)),
+                kvcache.workspace_views(self._ws[self._ws_off:], lay, T, H), cache, block_table, seq_lens, plan, max_new,
+                self.causal)
+            y = torch.empty_like(x)
+            _lib.check(L.b200l_outproj_res_ln(ctypes.byref(desc), x.data_ptr(), y.data_ptr(), self.workspace_ptr,
+                                              self._ws_bytes, st))
+        return y
 
     def _forward_reduced(self, x: torch.Tensor, valid_token_mask: Optional[torch.Tensor],
                          out: Optional[torch.Tensor]) -> torch.Tensor:

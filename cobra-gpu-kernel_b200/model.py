@@ -16,12 +16,12 @@ There is no CPU path: x must be fp32 on an sm_100 device.
 from __future__ import annotations
 
 import ctypes
-from typing import List, Optional
+from typing import List, Optional, Sequence
 
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _lib, kvcache
 from .layer import SelfAttentionWeights, TransformerConfig
 
 
@@ -184,13 +184,57 @@ class B200Transformer(nn.Module):
                 _lib.check(L.b200l_block_forward(ctypes.byref(desc), cur.data_ptr(), nxt.data_ptr(),
                                                  self.workspace_ptr, self._ws_bytes, stream))
                 cur = nxt
-            fw, fb = self.final_norm.weight, self.final_norm.bias
-            fw32 = fw.detach().to(device=dev, dtype=torch.float32).contiguous()
-            fb32 = fb.detach().to(device=dev, dtype=torch.float32).contiguous()
-            _lib.check(L.b200l_row_layernorm(cur.data_ptr(), cur.data_ptr(), fw32.data_ptr(), fb32.data_ptr(),
-                                             float(self.final_norm.eps), B * S, d,
-                                             mask.data_ptr() if mask is not None else None, stream))
+            self._final_norm(cur, mask, stream)
             return cur
+
+
+    # ------------------------------------------------------------ cached steps
+    def new_caches(self, num_pages: int, *, page_size: int = 64, dtype: torch.dtype = torch.int8,
+                   device="cuda") -> List[kvcache.KVCache]:
+        """An empty cache for every layer."""
+        dh = self.config.d_model // self.config.num_heads
+        return [kvcache.new_kv_cache(num_pages, self.config.num_heads, dh, page_size=page_size, dtype=dtype, device=device)
+                for _ in self.layers]
+
+    def forward_cached(self, x: torch.Tensor, caches: Sequence[kvcache.KVCache], block_table: torch.Tensor,
+                       seq_lens: torch.Tensor, plan: kvcache.KVPlan, *, max_new: int) -> torch.Tensor:
+        """The stack on new tokens alone, each layer attending to its cache
+        (``caches``, one per layer; all share the block table): x fp32 [tokens, d]
+        as in ``B200TransformerLayer.forward_cached``, the next token of every
+        request or chunks of their prompts. Returns a new tensor."""
+        d, H = self.config.d_model, self.config.num_heads
+        kvcache.check_step(x, d, plan)
+        if len(caches) != len(self.layers):
+            raise ValueError(f"{len(self.layers)} layers need as many caches, got {len(caches)}")
+        x = x.contiguous()
+        T, dev, L = x.shape[0], x.device, _lib.lib()
+        with torch.cuda.device(dev):
+            packs = self._ensure_packs(dev)
+            descs = [self._block_desc(blk, pk, 1, T, None) for blk, pk in zip(self.layers, packs)]
+            self._ensure_workspace(descs[0], dev)
+            st = torch.cuda.current_stream(dev).cuda_stream
+            views = kvcache.workspace_views(self._ws[self._ws_off:], _lib.workspace_layout(1, T, d, H), T, H)
+            bufs, cur = [torch.empty_like(x), torch.empty_like(x)], x
+            for i, (desc, cache) in enumerate(zip(descs, caches)):
+                nxt = bufs[i % 2]
+                kvcache.attend_cached(
+                    lambda: _lib.check(L.b200l_qkv_ln_gemm(ctypes.byref(desc.layer), cur.data_ptr(), self.workspace_ptr,
+                                                           self._ws_bytes, st)),
+                    views, cache, block_table, seq_lens, plan, max_new, self.config.causal)
+                _lib.check(L.b200l_block_finish(ctypes.byref(desc), cur.data_ptr(), nxt.data_ptr(), self.workspace_ptr,
+                                                self._ws_bytes, st))
+                cur = nxt
+            self._final_norm(cur, None, st)
+            return cur
+
+    def _final_norm(self, x: torch.Tensor, mask: Optional[torch.Tensor], stream: int) -> None:
+        """final_norm of x's rows, in place; rows whose mask byte is 0 become 0."""
+        d = x.shape[-1]
+        fw, fb = (t.detach().to(device=x.device, dtype=torch.float32).contiguous()
+                  for t in (self.final_norm.weight, self.final_norm.bias))
+        _lib.check(_lib.lib().b200l_row_layernorm(x.data_ptr(), x.data_ptr(), fw.data_ptr(), fb.data_ptr(),
+                                                  float(self.final_norm.eps), x.numel() // d, d,
+                                                  mask.data_ptr() if mask is not None else None, stream))
 
 
 def _validate_stack_config(config) -> None:

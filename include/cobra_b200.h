@@ -213,6 +213,13 @@ B200L_API size_t b200l_block_workspace_bytes(const b200l_block_desc* desc);
 B200L_API int b200l_block_forward(const b200l_block_desc* desc, const float* x, float* y,
                                   void* workspace, size_t ws_bytes, void* stream);
 
+/* The block from ctx (fp16 [T, d]) in the workspace on: x1 = x + ctx Wo^T + bo,
+ * then the FFN half. With b200l_qkv_ln_gemm before it and another attention in
+ * between (b200l_kv_attention) it makes the block of a cached step. Workspace as
+ * b200l_block_forward. */
+B200L_API int b200l_block_finish(const b200l_block_desc* desc, const float* x, float* y,
+                                 void* workspace, size_t ws_bytes, void* stream);
+
 /* y = LayerNorm(x) row by row (fp32 in/out, d a multiple of 4, at most 2048),
  * rows whose row_mask byte is 0 set to zero (row_mask may be NULL). x may equal
  * y. The stack's final_norm and its padded-row mask: replaces
