@@ -43,7 +43,7 @@ struct KvAppendArgs {
   int vec[2];                    // rows are read in 16-byte pieces
   const long long* slots;
   long long tokens, num_slots;
-  int type, dh, window, windows;
+  int type, dh, window, windows, pairs;   // pairs: (head, K or V) that a group does one after another
 };
 
 template <int KIND>
@@ -188,17 +188,13 @@ __global__ void __launch_bounds__(256, ESZ == 2 ? 4 : 3) kv_append_kernel(KvAppe
   const int warp = threadIdx.x >> 5, gw = warp % GW;
   __shared__ float s_max[2][8];
   const unsigned id = blockIdx.x * (8 / GW) + warp / GW;
-  const int win = (int)(id / (2u * a.c.heads));
+  const unsigned chunks = (2u * a.c.heads + a.pairs - 1) / a.pairs;
+  const int win = (int)(id / chunks), hk0 = (int)(id - win * chunks) * a.pairs;   // neighbours share tokens: their rows lie side by side
   if (win >= a.windows) return;
-  const int hk = (int)(id - win * (2u * a.c.heads));   // neighbours share tokens: their rows lie side by side
-  const int head = hk >> 1, which = hk & 1, P = a.c.page;
+  const int hk1 = min(hk0 + a.pairs, 2 * a.c.heads), P = a.c.page;
   const long long t0 = (long long)win * a.window;
   const int W = (int)min((long long)a.window, a.tokens - t0);
-  uint8_t* codes = which ? a.c.v : a.c.k;
-  float* scales = which ? a.c.v_scale : a.c.k_scale;
-  const void* x = a.x[which];
-  const long long st = a.st[which], sd = a.sd[which], xh = head * a.sh[which];
-  const int sub = lane / LPT, d0 = (lane % LPT) * 8, vec = a.vec[which];
+  const int sub = lane / LPT, d0 = (lane % LPT) * 8;
 
   // Whether token t leads a run (1), goes on the one before it (0), or has no slot (2).
   auto kind_of = [&](long long t) {
@@ -214,7 +210,7 @@ __global__ void __launch_bounds__(256, ESZ == 2 ? 4 : 3) kv_append_kernel(KvAppe
   }
   const bool share = __popcll(lead) <= (GW + 1) / 2;   // (group-uniform)
   const int wv = share ? gw : 0, nw = share ? GW : 1;
-  for (int nth = 0; lead; ++nth) {
+  for (int nth = 0, turn = 0; lead; ++nth) {
     const int i = __ffsll((long long)lead) - 1;
     lead &= lead - 1;
     if (!share && nth % GW != gw) continue;
@@ -234,7 +230,12 @@ __global__ void __launch_bounds__(256, ESZ == 2 ? 4 : 3) kv_append_kernel(KvAppe
     const long long slot = a.slots[t0 + i];
     const long long page = slot >> a.c.log2_page;
     const int place = (int)(slot & (P - 1));
-    float* sp = scales + page * a.c.heads + head;
+    for (int hk = hk0; hk < hk1; ++hk, ++turn) {
+    const int head = hk >> 1, which = hk & 1, vec = a.vec[which];
+    uint8_t* codes = which ? a.c.v : a.c.k;
+    const void* x = a.x[which];
+    const long long st = a.st[which], sd = a.sd[which], xh = head * a.sh[which];
+    float* sp = (which ? a.c.v_scale : a.c.k_scale) + page * a.c.heads + head;
     const float was = place ? *sp : 0.f;
     const long long row0 = (page * a.c.heads + head) << a.c.log2_page;
 
@@ -262,11 +263,11 @@ __global__ void __launch_bounds__(256, ESZ == 2 ? 4 : 3) kv_append_kernel(KvAppe
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (share) {                                  // (two buffers: the next run's maxima cannot overtake this one's readers)
-      if (lane == 0) s_max[nth & 1][warp] = m;
+    if (share) {                                  // (two buffers: the next turn's maxima cannot overtake this one's readers)
+      if (lane == 0) s_max[turn & 1][warp] = m;
       asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / GW), "n"(GW * 32) : "memory");
 #pragma unroll
-      for (int w = 0; w < GW; ++w) m = max_nan(m, s_max[nth & 1][warp / GW * GW + w]);
+      for (int w = 0; w < GW; ++w) m = max_nan(m, s_max[turn & 1][warp / GW * GW + w]);
     }
     const float want = kv_scale_for<KIND>(m);
     const float now = (want <= was || was != was) ? was : want;   // not-a-number stays
@@ -291,6 +292,7 @@ __global__ void __launch_bounds__(256, ESZ == 2 ? 4 : 3) kv_append_kernel(KvAppe
         if (j + sub < len)
           *reinterpret_cast<uint2*>(codes + (row0 + place + j + sub) * DHP + d0) = f[u].template codes<KIND>(now, inv, a.type);
       }
+    }
     }
   }
 }

@@ -98,7 +98,7 @@ int kv_plan_run(const b200l_kv_plan_desc* d, cudaStream_t st) {
 template <int DHP, int KIND>
 int kv_append_t(const KvAppendArgs& a, cudaStream_t st) {
   const int per = 8 / kv_append_group(DHP);      // groups of a block
-  const long long blocks = ((long long)a.windows * a.c.heads * 2 + per - 1) / per;
+  const long long blocks = ((long long)a.windows * ((a.c.heads * 2 + a.pairs - 1) / a.pairs) + per - 1) / per;
   if (blocks > 0x7fffffffLL) return fail(B200L_ERR_BAD_SHAPE, "kv_append: too many tokens and heads");
   cudaError_t e = a.type == B200L_DTYPE_F32
                       ? launch_pdl(kv_append_kernel<DHP, KIND, 4>, dim3((unsigned)blocks), dim3(256), 0, st, a)
@@ -163,6 +163,9 @@ int kv_append_run(const b200l_kv_cache* cache, const b200l_kv_rows* rows, const 
   a.window = gw;
   while (a.window < 64 && tokens * cache->num_heads * 2 / (a.window * 2) * gw >= 128ll * dev.sms) a.window *= 2;
   a.windows = (int)((tokens + a.window - 1) / a.window);
+  a.pairs = 1;                                    // beyond that, several heads a group
+  while (a.pairs < 8 && a.window == 64 && (long long)a.windows * cache->num_heads * 2 / (a.pairs * 2) * gw >= 128ll * dev.sms)
+    a.pairs *= 2;
 #define KV_CALL(D, K) kv_append_t<D, K>(a, st)
   KV_DISPATCH(cache->head_dim, cache->kind, KV_CALL)
 #undef KV_CALL
@@ -179,7 +182,9 @@ int kv_read_run(const b200l_kv_cache* cache, const int64_t* slots, int64_t n, vo
   if ((rc = device_info(&dev))) return rc;
   if (n == 0) return B200L_OK;
   if (!slots || !k_out || !v_out) return fail(B200L_ERR_NULL_POINTER, "kv_read: NULL pointer");
-  if (misaligned(k_out, 16) || misaligned(v_out, 16)) return fail(B200L_ERR_ALIGNMENT, "kv_read: outputs must be 16-byte aligned");
+  const size_t align = cache->head_dim % 8 == 0 ? 16 : dtype == B200L_DTYPE_F32 ? 4 : 2;   // rows in 16-byte pieces, or element by element
+  if (misaligned(k_out, align) || misaligned(v_out, align))
+    return fail(B200L_ERR_ALIGNMENT, "kv_read: outputs must be %zu-byte aligned", align);
   a.slots = reinterpret_cast<const long long*>(slots);
   a.out[0] = k_out;
   a.out[1] = v_out;

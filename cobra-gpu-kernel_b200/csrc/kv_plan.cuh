@@ -41,39 +41,52 @@ struct KvPlanArgs {
   int requests, width, page, log2_page, capacity, max_tokens;
 };
 
-// Exclusive sums of four counts over the block's threads; totals in tot.
-__device__ __forceinline__ void block_scan4(long long (&v)[4], long long (&tot)[4], long long (*part)[4]) {
+// Exclusive sums over the block's threads, totals in tot: of tokens (64 bits) and of
+// three counts of pages.
+struct KvSums {
+  long long tokens;
+  int take, give, pages;
+};
+__device__ __forceinline__ KvSums operator+(KvSums a, const KvSums& b) {
+  a.tokens += b.tokens;
+  a.take += b.take;
+  a.give += b.give;
+  a.pages += b.pages;
+  return a;
+}
+__device__ __forceinline__ KvSums warp_scan(KvSums v, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    KvSums y;
+    y.tokens = __shfl_up_sync(0xffffffffu, v.tokens, o);
+    y.take = __shfl_up_sync(0xffffffffu, v.take, o);
+    y.give = __shfl_up_sync(0xffffffffu, v.give, o);
+    y.pages = __shfl_up_sync(0xffffffffu, v.pages, o);
+    if (lane >= o) v = v + y;
+  }
+  return v;
+}
+__device__ __forceinline__ void block_scan(KvSums& v, KvSums& tot, KvSums* part) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  long long inc[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    long long x = v[c];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    inc[c] = x;
-    if (lane == 31) part[warp][c] = x;
+  const KvSums inc = warp_scan(v, lane);
+  if (lane == 31) part[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    const KvSums s = warp_scan(lane < nw ? part[lane] : KvSums{0, 0, 0, 0}, lane);
+    __syncwarp();
+    part[lane] = s;
   }
   __syncthreads();
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    long long before = 0, all = 0;
-    for (int w = 0; w < nw; ++w) {
-      const long long p = part[w][c];
-      if (w < warp) before += p;
-      all += p;
-    }
-    v[c] = before + inc[c] - v[c];
-    tot[c] = all;
-  }
+  const KvSums before = warp ? part[warp - 1] : KvSums{0, 0, 0, 0};
+  tot = part[nw - 1];
+  v = KvSums{before.tokens + inc.tokens - v.tokens, before.take + inc.take - v.take, before.give + inc.give - v.give,
+             before.pages + inc.pages - v.pages};
 }
 
 __global__ void __launch_bounds__(1024) kv_plan_kernel(KvPlanArgs a) {
   pdl_wait_then_release();
   extern __shared__ int sm_plan[];
-  __shared__ long long part[32][4];
+  __shared__ KvSums part[32];
   __shared__ unsigned long long s_over;
   const int R = a.requests;
   int* s_new = sm_plan;              // exclusive sums, R + 1 each: new tokens,
@@ -85,36 +98,30 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(KvPlanArgs a) {
 
   const int per = (R + blockDim.x - 1) / blockDim.x;
   const int r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
-  long long v[4] = {0, 0, 0, 0}, tot[4];
+  KvSums v{0, 0, 0, 0}, tot;
   long long over = 0;                // pages past the table's width
   for (int r = r0; r < r1; ++r) {
     const int o = length(a.old_lens, r), n = length(a.new_lens, r), po = pages(o), pn = pages(n);
-    v[0] += max(n - o, 0);
-    v[1] += max(pn - po, 0);
-    v[2] += max(po - pn, 0);
-    v[3] += n > o ? pn : 0;
+    v = v + KvSums{max(n - o, 0), max(pn - po, 0), max(po - pn, 0), n > o ? pn : 0};
     if (blockIdx.x == 0 && a.new_lens[r] > cap) over += ((long long)a.new_lens[r] + mask) / a.page - a.width;
   }
   if (threadIdx.x == 0) s_over = 0;
-  block_scan4(v, tot, part);
+  block_scan(v, tot, part);
   if (over) atomicAdd(&s_over, (unsigned long long)over);
   auto clip = [](long long x) { return (int)(x < 0x7fffffffLL ? x : 0x7fffffffLL); };
   const bool first = blockIdx.x == 0;
   for (int r = r0; r < r1; ++r) {
     const int o = length(a.old_lens, r), n = length(a.new_lens, r), po = pages(o), pn = pages(n);
-    s_new[r] = clip(v[0]);
-    s_take[r] = clip(v[1]);
-    s_give[r] = clip(v[2]);
+    s_new[r] = clip(v.tokens);
+    s_take[r] = v.take;
+    s_give[r] = v.give;
     if (first) {
-      a.cu_new[r] = clip(v[0]);
-      a.cu_pages[r] = clip(v[3]);
+      a.cu_new[r] = clip(v.tokens);
+      a.cu_pages[r] = v.pages;
     }
-    v[0] += max(n - o, 0);
-    v[1] += max(pn - po, 0);
-    v[2] += max(po - pn, 0);
-    v[3] += n > o ? pn : 0;
+    v = v + KvSums{max(n - o, 0), max(pn - po, 0), max(po - pn, 0), n > o ? pn : 0};
   }
-  const int total = clip(tot[0]), take = clip(tot[1]), give = clip(tot[2]);
+  const int total = clip(tot.tokens), take = tot.take, give = tot.give;
   const int count = min(max(*a.free_count, 0), a.capacity), top = count + give;
   if (threadIdx.x == 0) {
     s_new[R] = total;
@@ -122,7 +129,7 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(KvPlanArgs a) {
     s_give[R] = give;
     if (first) {
       a.cu_new[R] = total;
-      a.cu_pages[R] = clip(tot[3]);
+      a.cu_pages[R] = tot.pages;
     }
   }
   __syncthreads();

@@ -150,16 +150,19 @@ def _cache_desc(cache: KVCache, head_dim: int, index: int) -> bytes:
 # ---------------------------------------------------------------- workspaces
 class _Workspace:
     """A workspace of each (device, stream): calls on one stream run one after
-    another, so they can share it. A buffer that was outgrown is kept (a captured
-    graph may still use it); each is at least twice the one before."""
+    another, so they can share it. (Graphs captured on one stream share it too and
+    are not to be replayed at the same time.) A buffer that was outgrown is kept (a
+    captured graph may still use it); each is at least twice the one before. One
+    that was made during a capture has its status block cleared by every call: the
+    clearing that made it usable is in that graph, not in the stream."""
 
     def __init__(self) -> None:
         self._held: Dict[Tuple[int, int], list] = {}
 
-    def get(self, index: int, stream: int) -> Tuple[int, int]:
-        """(address, bytes), 0 bytes if there is none yet."""
+    def get(self, index: int, stream: int) -> Tuple[int, int, bool]:
+        """(address, bytes, to be cleared), 0 bytes if there is none yet."""
         held = self._held.get((index, stream))
-        return held[-1][:2] if held else (0, 0)
+        return held[-1][:3] if held else (0, 0, False)
 
     def grow(self, index: int, stream: int, need: int) -> Tuple[int, int]:
         held = self._held.setdefault((index, stream), [])
@@ -167,13 +170,13 @@ class _Workspace:
         buf = torch.empty(size + 1024, dtype=torch.uint8, device=torch.device("cuda", index))
         ptr = (buf.data_ptr() + 1023) // 1024 * 1024
         _lib.check(_lib.lib().b200l_clear_status(ptr, stream))
-        held.append((ptr, size, buf))
+        held.append((ptr, size, torch.cuda.is_current_stream_capturing(), buf))
         return ptr, size
 
     def check(self) -> None:
         for (index, stream), held in self._held.items():
             with torch.cuda.device(index):
-                for ptr, _, _ in held:
+                for ptr, _, _, _ in held:
                     rc = _lib.lib().b200l_read_status(ptr, stream)
                     if rc:
                         message = _lib.last_error()
@@ -192,7 +195,7 @@ def kv_check_status() -> None:
 
 def _on_device(call, index: int, *args):
     """call(stream, *args) with device ``index`` current and its current stream."""
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         return call(torch._C._cuda_getCurrentRawStream(index), *args)
     with torch.cuda.device(index):
         return call(torch._C._cuda_getCurrentRawStream(index), *args)
@@ -238,9 +241,10 @@ def kv_plan(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.T
 def _plan(stream, old_lens, new_lens, table, stride, free_pages, free_count, page_size, max_tokens) -> KVPlan:
     R, width = table.shape
     # One allocation: slots (8 bytes each), then the int32 outputs.
-    buf = torch.empty(3 * max_tokens + 2 * R + 4, dtype=torch.int32, device=old_lens.device)
+    buf = old_lens.new_empty(3 * max_tokens + 2 * R + 4)
     at = buf.data_ptr()
-    slots, positions, cu_new, cu_pages, info = buf.split_with_sizes((2 * max_tokens, max_tokens, R + 1, R + 1, 2))
+    slots, positions, cu_new, cu_pages, info = torch.unsafe_split_with_sizes(
+        buf, (2 * max_tokens, max_tokens, R + 1, R + 1, 2))
     p_pos = at + 8 * max_tokens
     p_new = p_pos + 4 * max_tokens
     p_pages = p_new + 4 * (R + 1)
@@ -309,8 +313,7 @@ def kv_read(slots: torch.Tensor, cache: KVCache, head_dim: int, *,
 
 def _read(stream, c, slots, heads, dh, dtype, code) -> Tuple[torch.Tensor, torch.Tensor]:
     n = slots.shape[0]
-    k = torch.empty((n, heads, dh), dtype=dtype, device=slots.device)
-    v = torch.empty_like(k)
+    k, v = slots.new_empty((2, n, heads, dh), dtype=dtype).unbind()
     if n:
         rc = _lib.lib().b200l_kv_read(c, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code, stream)
         if rc:
@@ -358,7 +361,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq
                          f"{cu_new.numel()}, {cu_pages.numel()}")
     stride = _table_stride(block_table, R)
     if out is None:
-        out = torch.empty((T, hq, dh), dtype=dtype, device=q.device)
+        out = q.new_empty((T, hq, dh))
     elif out.shape != q.shape or out.dtype != dtype or out.get_device() != index or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     if T == 0:
@@ -373,7 +376,9 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq
 
 def _attention(stream, index, c, desc) -> None:
     L = _lib.lib()
-    ws, size = _workspace.get(index, stream)
+    ws, size, clear = _workspace.get(index, stream)
+    if clear:
+        _lib.check(L.b200l_clear_status(ws, stream))
     rc = L.b200l_kv_attention(c, desc, ws, size, stream)
     if rc == _lib.ERR_WORKSPACE:
         need = L.b200l_kv_attention_workspace_bytes(c, desc)

@@ -360,8 +360,8 @@ B200L_API int b200l_kv_append(const b200l_kv_cache* cache, const b200l_kv_rows* 
                               int64_t tokens, void* stream);
 
 /* The values of n slots, code * scale rounded once to dtype: k_out and v_out
- * are [n, num_heads, head_dim], contiguous, 16-byte aligned. Slots outside the
- * cache read as 0. */
+ * are [n, num_heads, head_dim], contiguous, 16-byte aligned where head_dim is a
+ * multiple of 8. Slots outside the cache read as 0. */
 B200L_API int b200l_kv_read(const b200l_kv_cache* cache, const int64_t* slots, int64_t n, void* k_out, void* v_out,
                             int32_t dtype, void* stream);
 

@@ -480,6 +480,25 @@ def test_step_in_a_graph(pkg, cuda_ok):
         count.copy_(plan.info[:1])
 
 
+def test_second_graph_before_the_first(pkg, cuda_ok):
+    """Two graphs share the workspace that the first capture made; the second one's replay comes first."""
+    s = attention_case(pkg, 20, "int8", "fp16", 4, 2, 64, 16, [90, 3000, 7], [1, 1, 1])
+    want = check_attention(pkg, s)
+    plan = pkg.KVPlan(i32(s["cu"]), i32(s["cup"]), None, None, None)
+    q, table, lens = s["q"].cuda(), i32(s["table"]), i32(s["lens"])
+    side, outs, graphs = torch.cuda.Stream(), [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append(pkg.kv_attention(q, s["c"], table, lens, plan, max_new=1))
+    for i in (1, 0):
+        outs[i].zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want)
+    pkg.kv_check_status()
+
+
 def test_refusals(pkg, cuda_ok):
     """What Python refuses before the library is asked, with the reason."""
     c = pkg.new_kv_cache(4, 2, 64, page_size=16)
