@@ -27,7 +27,7 @@
 // be worth it, stretches are whole pairs and there is nothing to join.
 //
 // Products are mma.sync m16n8k16: one tile of M rows has too little work for
-// tcgen05 (2 FLOP per byte read and row; HBM bounds it below M ~ 250). The
+// tcgen05 (2 FLOP per byte read and row; HBM bounds it below M ~ 130). The
 // transposed products are taken, S^T = K Q^T and O^T = V^T P^T, so that the 16
 // of the shape are keys or dims, always full, and the 8 are rows: a token's few
 // query heads pad to 8, and accumulators, Q and exponentials are half of what
