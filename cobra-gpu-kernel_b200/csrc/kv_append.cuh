@@ -29,7 +29,10 @@
 // Bound: HBM, 2 (or 4) bytes read and 1 written per value. A run is a chain of
 // some 3000 clocks (slots, values and scale, maximum, codes), so about 45 KB of
 // values have to be on their way in an SM: 32 warps of 2 KB. A decode step is
-// that chain once.
+// that chain once. Measured: 65536 prompt tokens, 16 heads of 64, fp16 to e4m3 122
+// us (403 MB, 51 % of HBM's rate: instructions a value); 6077 tokens of 24 ragged
+// prompts, 8 heads of 128, bf16 to int8 29 us (the chain, on too few runs); 64
+// single tokens, 4 heads of 32, 4.4 us.
 #pragma once
 
 #include "kv_common.cuh"
@@ -307,7 +310,7 @@ struct KvReadArgs {
 
 // Value = code * scale, rounded once; slots outside the cache read as 0.
 // A lane takes 8 codes of a token and head, K and V alike, two pieces at a time.
-// Bound: HBM.
+// Bound: HBM; 65536 tokens, 16 heads of 64, e4m3 to fp16 88 us (403 MB, 71 %).
 template <int DHP, int KIND>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvReadArgs a) {
   pdl_wait_then_release();

@@ -26,6 +26,11 @@
 // leave a piece adding them itself, 8 us). Where tables are too narrow for it to
 // be worth it, stretches are whole pairs and there is nothing to join.
 //
+// Measured: 256 requests of about 7000 tokens, 32 / 8 heads of 128, int8 585-610 us
+// (3.7 GB, 94-98 % of HBM's rate); 2 requests of 100000, 16 heads of 64, e4m3 81 us
+// (77 %); 64 ragged requests, 32 / 8 heads of 128 105 us (76 %): the rest is the
+// first loads' latency, the join, and warps that end apart.
+//
 // Products are mma.sync m16n8k16: one tile of M rows has too little work for
 // tcgen05 (2 FLOP per byte read and row; HBM bounds it below M ~ 130). The
 // transposed products are taken, S^T = K Q^T and O^T = V^T P^T, so that the 16

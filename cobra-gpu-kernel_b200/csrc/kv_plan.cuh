@@ -18,8 +18,9 @@
 // entries lie past the old ones. So a repeated call gives the same answer, and
 // the caller keeps a step by adopting its lengths and its count of free pages.
 //
-// Bound: one pass over the lists (12 bytes a token written), at small sizes
-// the launch and one block's scan.
+// Bound: latency. 32 requests with a token each take 2.4 us (launch and one block's
+// sums), 4096 requests with 281 thousand new tokens 12 us, of which writing the 12
+// bytes a token would be 0.7.
 #pragma once
 
 #include "kv_common.cuh"

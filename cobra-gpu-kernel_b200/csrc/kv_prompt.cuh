@@ -33,6 +33,9 @@
 //
 // Bound: exponentials and products alike at dhp 128 (16 per clock and SM, 2048
 // clocks a 256 x 128 tile, and 4 x 512 clocks of tcgen05), exponentials below.
+// Measured at 32768 keys and 1024 rows a head: 540-560 TFLOP/s at dhp 64 (4400
+// clocks a tile), 740-800 at 128, 490-590 at 256; the tile is held up by issue slots
+// (10000 instructions) and their fetching, which is why code stays small here.
 #pragma once
 
 #include "kv_decode.cuh"
