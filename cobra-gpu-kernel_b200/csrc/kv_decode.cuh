@@ -26,9 +26,9 @@
 // leave a piece adding them itself, 8 us). Where tables are too narrow for it to
 // be worth it, stretches are whole pairs and there is nothing to join.
 //
-// Measured: 256 requests of about 7000 tokens, 32 / 8 heads of 128, int8 585-610 us
-// (3.7 GB, 94-98 % of HBM's rate); 2 requests of 100000, 16 heads of 64, e4m3 81 us
-// (77 %); 64 ragged requests, 32 / 8 heads of 128 105 us (76 %): the rest is the
+// Measured: 256 requests of about 7000 tokens, 32 / 8 heads of 128, int8 585-654 us
+// (3.7 GB, 88-98 % of HBM's rate); 2 requests of 100000, 16 heads of 64, e4m3 82-86 us
+// (74-77 %); 64 ragged requests, 32 / 8 heads of 128 106-108 us (75 %): the rest is the
 // first loads' latency, the join, and warps that end apart.
 //
 // Products are mma.sync m16n8k16: one tile of M rows has too little work for

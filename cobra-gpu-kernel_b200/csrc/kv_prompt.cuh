@@ -33,9 +33,12 @@
 //
 // Bound: exponentials and products alike at dhp 128 (16 per clock and SM, 2048
 // clocks a 256 x 128 tile, and 4 x 512 clocks of tcgen05), exponentials below.
-// Measured at 32768 keys and 1024 rows a head: 540-560 TFLOP/s at dhp 64 (4400
-// clocks a tile), 740-800 at 128, 490-590 at 256; the tile is held up by issue slots
-// (10000 instructions) and their fetching, which is why code stays small here.
+// Measured (int8, 32768 keys, 1024 rows a head, 512 at dhp 256): 275 TFLOP/s at dhp
+// 32, 542 at 64 (4350 clocks a tile), 764 at 128, 504 at 256. Blocks that took
+// every so many'th item, with the softmax in unrolled passes, reached 293, 545, 797
+// and 586, and 103 against 112 us on 8 prompts of 960, 16 heads of 64; the even cut
+// with the rolled pass takes 673 against 743 us on 6 chunks of unlike length, 32 / 8
+// heads of 128. Issue slots are 59 % full on those.
 #pragma once
 
 #include "kv_decode.cuh"
