@@ -11,7 +11,10 @@
 // that multiply codes are at most 2^8 and go into fp16 relative to the largest
 // contribution, and no accumulator is rescaled per page. Sums and maxima are
 // fp32; fp16 rounds q (scaled by a power of two to [1, 2) at the row's largest
-// if it comes as bf16: exact but for what is 2^-14 of it) and the weights.
+// if it comes as bf16: exact but for what is 2^-14 of it) and the weights of the
+// numerator: to 2^-12 of themselves, below 2^-14 to 2^-25 of the largest
+// contribution. The denominator must not lose those, for there a key counts with
+// 2^t whatever its values' size: it sums the weights in fp32.
 //
 // Bound: HBM, 2 dhp bytes per cached token and head. Work is split evenly over
 // warps, not requests: the keys of all (request, head) pairs in a row are cut
@@ -40,9 +43,10 @@
 // free as long as both operands agree, so fragments are read straight from the
 // page's rows: as A of K Q^T a lane takes 16 consecutive code bytes of a key; as A
 // of V^T P^T the same bytes of four keys, transposed by byte permutes on the way
-// to fp16. P^T goes from accumulator to operand by movmatrix. The row sums are a
-// product with ones, of the weights as fp16 has them, so that what rounds a
-// weight rounds it above and below alike.
+// to fp16. P^T goes from accumulator to operand by movmatrix. The row sums take
+// the weights rounded to fp16's 11 bits, so that what rounds a weight rounds it
+// above and below alike, but with fp32's exponent; a lane sums its own keys, and
+// lanes are added once a pair.
 #pragma once
 
 #include "kv_common.cuh"
@@ -183,6 +187,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A weight as fp16 has it where it is 2^-14 or more, and to as many bits where it
+// is less. (A not-a-number may come out as 0: the product with V has it.)
+__device__ __forceinline__ float round11(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
 }
 
 // Transposes an 8 x 8 tile of 16-bit values, two of a row a lane.
@@ -519,13 +529,12 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
         const float m0 = mx[m][0] == -INFINITY ? 0.f : mx[m][0], m1 = mx[m][1] == -INFINITY ? 0.f : mx[m][1];
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-          p[j][m][0] = transpose8x8(pack_half2(ex2_approx(acc[j][m][0] - m0), ex2_approx(acc[j][m][1] - m1)));
-          p[j][m][1] = transpose8x8(pack_half2(ex2_approx(acc[j][m][2] - m0), ex2_approx(acc[j][m][3] - m1)));
-          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(sum, ones, p[j][m][0], p[j][m][1]);
-          l[m][0] = fmaf(sum[0], inv[j], l[m][0]);
-          l[m][1] = fmaf(sum[1], inv[j], l[m][1]);
+          const float e0 = ex2_approx(acc[j][m][0] - m0), e1 = ex2_approx(acc[j][m][1] - m1);
+          const float e2 = ex2_approx(acc[j][m][2] - m0), e3 = ex2_approx(acc[j][m][3] - m1);
+          p[j][m][0] = transpose8x8(pack_half2(e0, e1));
+          p[j][m][1] = transpose8x8(pack_half2(e2, e3));
+          l[m][0] = fmaf(round11(e0) + round11(e2), inv[j], l[m][0]);
+          l[m][1] = fmaf(round11(e1) + round11(e3), inv[j], l[m][1]);
         }
       }
       // ---- O^T += V^T P^T, 16 keys a step
@@ -582,6 +591,13 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
       issue();
     }
     if (!ok) break;
+#pragma unroll
+    for (int m = 0; m < NR; ++m)
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2) {           // the sums of this lane's keys -> of all
+        l[m][0] += __shfl_xor_sync(0xffffffffu, l[m][0], x);
+        l[m][1] += __shfl_xor_sync(0xffffffffu, l[m][1], x);
+      }
 
     // ---- the pair's result, or this piece of it: dims [VB g, VB g + VB) of each box
     const bool whole = sp.p0 == 0 && sp.p1 == sp.nu;

@@ -1,0 +1,55 @@
+"""The paged 8-bit cache on a B200 where a step's numbers lie apart or its calls are at odds."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests import kv_reference as ref
+from tests.test_kvcache_gpu import KIND, TOL, attention_case, i32, run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- value scales far apart
+def unlike_pages(s, small, order):
+    """Values of one size throughout a page: full pages, and pages `small` times
+    theirs (0: nothing but zeros, as kv_append leaves them). Keys and queries stay."""
+    full = 100 if s["kind"] == "int8" else int(np.flatnonzero(ref._E4M3[:127] == 256.0)[0])
+    dh, at = s["dh"], 0
+    for row in s["table"]:
+        ids = [i for i in row if i >= 0]
+        for k, page in enumerate(ids):
+            is_full = {"full first": k == 0, "full last": k == len(ids) - 1, "in turn": k % 2 == at % 2}[order]
+            s["vc"][page] = 0
+            if is_full or small:
+                s["vc"][page, :, :, :dh] = full
+            s["vs"][page] = np.float32(2.0 ** -6 * (1.0 if is_full else small))
+        at += 1
+    s["c"].v.view(torch.uint8).copy_(torch.from_numpy(s["vc"]))
+    s["c"].v_scale.copy_(torch.from_numpy(s["vs"]))
+
+
+@pytest.mark.parametrize("order", ["full first", "full last", "in turn"])
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -16, 2.0 ** -20, 2.0 ** -24])
+@pytest.mark.parametrize("kind,dtype,hq,hkv,dh,P", [
+    ("int8", "fp16", 4, 4, 32, 16), ("fp8", "bf16", 8, 2, 64, 16), ("int8", "fp16", 8, 2, 128, 32), ("fp8", "fp16", 2, 1, 256, 16)])
+def test_attention_counts_keys_of_small_values(pkg, cuda_ok, kind, dtype, hq, hkv, dh, P, small, order):
+    """A key's weight in the denominator is its own, however small its values: two
+    pages in one key tile, pages in several, and a context cut over the whole GPU, by
+    the kernel for few rows and by the one for many.
+
+    All values are of one sign, so the error is bounded by the output itself: what
+    rounds as in TOL, and besides the fp16 weights of the small pages' keys, off by up
+    to 2^-25 of the largest, 3100 of them at most: below 2^-13."""
+    for lens, new in (([2 * P], [1]), ([2 * P], [5]), ([2 * P + 40], [40]), ([7 * P - 3, 2 * P, 3 * P], [1, 1, 1]),
+                      ([3100], [1]), ([700, P + 1], [40, 1])):
+        for spread in (0.0, 1.0):
+            s = attention_case(pkg, 21 + dh, kind, dtype, hq, hkv, dh, P, lens, new, spread=spread)
+            unlike_pages(s, small, order)
+            got = run_attention(pkg, s)
+            pkg.kv_check_status()
+            want, _ = ref.attention(s["q"].double().numpy(), s["kc"], s["vc"], s["ks"], s["vs"], s["kind"], s["table"],
+                                    s["lens"], s["cu"], s["causal"], dh ** -0.5)
+            err = np.abs(got.double().cpu().numpy() - want)
+            bound = (TOL[dtype] + 2.0 ** -13) * np.abs(want) + (2.0 ** -25 if dtype == "fp16" else 0.0)   # fp16's least step
+            assert (err <= bound).all(), f"{lens} {new} {spread}: {(err / np.abs(want).clip(1e-30)).max():.3g} of the output"
