@@ -228,14 +228,15 @@ class B200TransformerLayer(nn.Module):
     def _ensure_workspace(self, desc: _lib.LayerDesc, device: torch.device, stepwise: bool = False) -> None:
         """Grow the workspace to what ``b200l_layer_forward`` needs for this
         shape (the status block alone for the whole-layer kernel), or with
-        ``stepwise`` to what the per-kernel entry points need."""
+        ``stepwise`` to what the per-kernel entry points need. The captured
+        graph goes with the workspace that it was captured on."""
         L = _lib.lib()
         fn = L.b200l_kernel_workspace_bytes if stepwise else L.b200l_layer_workspace_bytes
         need = fn(ctypes.byref(desc))
         if need == 0:
             raise _lib.B200LError(-1, _lib.last_error())
         if self._ws is None or self._ws.device != device or self._ws_bytes < need:
-            self._ws = None
+            self._ws = self._graph = None
             buf = torch.empty(need + 1024, dtype=torch.uint8, device=device)
             off = (-buf.data_ptr()) % 1024
             self._ws, self._ws_off, self._ws_bytes = buf, off, need

@@ -53,3 +53,29 @@ def test_attention_counts_keys_of_small_values(pkg, cuda_ok, kind, dtype, hq, hk
             err = np.abs(got.double().cpu().numpy() - want)
             bound = (TOL[dtype] + 2.0 ** -13) * np.abs(want) + (2.0 ** -25 if dtype == "fp16" else 0.0)   # fp16's least step
             assert (err <= bound).all(), f"{lens} {new} {spread}: {(err / np.abs(want).clip(1e-30)).max():.3g} of the output"
+
+
+# ---------------------------------------------------------------- workspaces of cached steps
+def one_prompt(pkg, S, d, H, P=16):
+    """Pool, cache, lengths and plan of one request's first S tokens."""
+    pool = pkg.KVPool(1, ref.ceil_div(S, P) + 1, ref.ceil_div(S, P) + 1, page_size=P)
+    lens = i32([S])
+    return pool, pkg.new_kv_cache(ref.ceil_div(S, P) + 1, H, d // H, page_size=P), lens, pool.plan(lens, S)
+
+
+@pytest.mark.parametrize("d,H,B,S", [(128, 4, 2, 16), (256, 4, 2, 40), (1024, 16, 1, 64)])
+def test_forward_before_and_after_a_larger_cached_step(pkg, cuda_ok, d, H, B, S):
+    """The layer's captured graph does not outlive the workspace that it was captured on."""
+    torch.manual_seed(d)
+    lay = pkg.B200TransformerLayer(d, H, True).cuda().eval()
+    x, long = torch.randn(B, S, d, device="cuda"), torch.randn(900, d, device="cuda")
+    with torch.inference_mode():
+        want = lay(x).clone()
+        lay(x)
+        pool, cache, lens, plan = one_prompt(pkg, 900, d, H)
+        lay.forward_cached(long, cache, pool.block_table, lens, plan, max_new=900)
+        others = [torch.full((1 << k,), 7, dtype=torch.uint8, device="cuda") for k in range(8, 23)]
+        for _ in range(2):
+            assert torch.equal(lay(x), want)
+        assert all(bool((t == 7).all()) for t in others)
+        lay.check_status()
