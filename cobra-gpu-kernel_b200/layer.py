@@ -32,6 +32,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, kvcache
+from .workspace import HoldsWorkspace
 
 GRAPH_MAX_INPUT_BYTES = 64 * 1024 * 1024   # reference gate, torch_transformer_benchmark.py:1077-1079
 _REDUCED = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}   # converted at the boundary
@@ -118,7 +119,7 @@ class _Pack:
     __slots__ = ("wqkv16", "bqkv32", "wo16", "ln", "device", "versions")
 
 
-class B200TransformerLayer(nn.Module):
+class B200TransformerLayer(HoldsWorkspace, nn.Module):
     """LN1 -> MHA -> +x -> LN2 on B200, with the reference's API.
 
     ``forward(x, valid_token_mask=None)``: x is fp32 [B, S, d] on an sm_100
@@ -145,9 +146,6 @@ class B200TransformerLayer(nn.Module):
         self.attention = SelfAttentionWeights(d_model, num_heads)
         self.norm2 = nn.LayerNorm(d_model)
         self._pack: Optional[_Pack] = None
-        self._ws: Optional[torch.Tensor] = None
-        self._ws_off = 0
-        self._ws_bytes = 0
         self._sig = None
         self._graph = None
         self._static_x = None
@@ -235,18 +233,8 @@ class B200TransformerLayer(nn.Module):
         need = fn(ctypes.byref(desc))
         if need == 0:
             raise _lib.B200LError(-1, _lib.last_error())
-        if self._ws is None or self._ws.device != device or self._ws_bytes < need:
-            self._ws = self._graph = None
-            buf = torch.empty(need + 1024, dtype=torch.uint8, device=device)
-            off = (-buf.data_ptr()) % 1024
-            self._ws, self._ws_off, self._ws_bytes = buf, off, need
-            with torch.cuda.device(device):
-                _lib.check(L.b200l_clear_status(self.workspace_ptr,
-                                                torch.cuda.current_stream(device).cuda_stream))
-
-    @property
-    def workspace_ptr(self) -> int:
-        return self._ws.data_ptr() + self._ws_off
+        if self._hold_workspace(need, device):
+            self._graph = None
 
     # ------------------------------------------------------------ compute
     def _launch(self, x: torch.Tensor, y: torch.Tensor, desc: _lib.LayerDesc) -> None:
@@ -254,16 +242,6 @@ class B200TransformerLayer(nn.Module):
         stream = torch.cuda.current_stream(x.device).cuda_stream
         _lib.check(L.b200l_layer_forward(ctypes.byref(desc), x.data_ptr(), y.data_ptr(),
                                          self.workspace_ptr, self._ws_bytes, stream))
-
-    def check_status(self) -> None:
-        """Synchronise and raise if a kernel recorded a device-side failure."""
-        if self._ws is None:
-            return
-        L = _lib.lib()
-        with torch.cuda.device(self._ws.device):
-            rc = L.b200l_read_status(self.workspace_ptr,
-                                     torch.cuda.current_stream(self._ws.device).cuda_stream)
-        _lib.check(rc)
 
     # ------------------------------------------------------------ head sharding
     def _head_pack(self, device: torch.device, h0: int, h1: int):

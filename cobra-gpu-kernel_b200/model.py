@@ -23,6 +23,7 @@ import torch.nn as nn
 
 from . import _lib, kvcache
 from .layer import SelfAttentionWeights, TransformerConfig
+from .workspace import HoldsWorkspace
 
 
 class B200TransformerBlock(nn.Module):
@@ -42,7 +43,7 @@ class _BlockPack:
     __slots__ = ("tensors", "desc")
 
 
-class B200Transformer(nn.Module):
+class B200Transformer(HoldsWorkspace, nn.Module):
     """``num_layers`` encoder blocks + ``final_norm`` on B200.
 
     ``forward(x, valid_token_mask=None)``: x fp32 [B, S, d] on the device that
@@ -60,9 +61,6 @@ class B200Transformer(nn.Module):
         self.final_norm = nn.LayerNorm(config.d_model)
         self._packs: Optional[List[_BlockPack]] = None
         self._pack_key = None
-        self._ws: Optional[torch.Tensor] = None
-        self._ws_off = 0
-        self._ws_bytes = 0
         self.register_load_state_dict_post_hook(lambda mod, _keys: mod.invalidate())
 
     def invalidate(self) -> None:
@@ -132,25 +130,7 @@ class B200Transformer(nn.Module):
         need = L.b200l_block_workspace_bytes(ctypes.byref(desc))
         if need == 0:
             raise _lib.B200LError(-1, _lib.last_error())
-        if self._ws is None or self._ws.device != device or self._ws_bytes < need:
-            self._ws = None
-            buf = torch.empty(need + 1024, dtype=torch.uint8, device=device)
-            self._ws, self._ws_off, self._ws_bytes = buf, (-buf.data_ptr()) % 1024, need
-            with torch.cuda.device(device):
-                _lib.check(L.b200l_clear_status(self.workspace_ptr, torch.cuda.current_stream(device).cuda_stream))
-
-    @property
-    def workspace_ptr(self) -> int:
-        return self._ws.data_ptr() + self._ws_off
-
-    def check_status(self) -> None:
-        """Synchronise and raise if a kernel recorded a device-side failure."""
-        if self._ws is None:
-            return
-        with torch.cuda.device(self._ws.device):
-            rc = _lib.lib().b200l_read_status(self.workspace_ptr,
-                                              torch.cuda.current_stream(self._ws.device).cuda_stream)
-        _lib.check(rc)
+        self._hold_workspace(need, device)
 
     # ------------------------------------------------------------ forward
     def forward(self, x: torch.Tensor, valid_token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:

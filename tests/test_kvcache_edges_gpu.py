@@ -79,3 +79,37 @@ def test_forward_before_and_after_a_larger_cached_step(pkg, cuda_ok, d, H, B, S)
             assert torch.equal(lay(x), want)
         assert all(bool((t == 7).all()) for t in others)
         lay.check_status()
+
+
+@pytest.mark.parametrize("stack", [False, True])
+def test_captured_cached_step_after_a_larger_one(pkg, cuda_ok, stack):
+    """A caller's graph of a cached step, replayed after an eager step that needed a larger
+    workspace: the same values, and no other tensor touched."""
+    d, H, S, P = 256, 4, 20, 16
+    torch.manual_seed(5)
+    if stack:
+        model = pkg.B200Transformer(pkg.TransformerConfig(1, 8, d, H, ffn_dim=512, num_layers=2, causal=True)).cuda().eval()
+        caches = model.new_caches(S // P + 2, page_size=P)
+    else:
+        model = pkg.B200TransformerLayer(d, H, True).cuda().eval()
+    pool, cache, lens, plan = one_prompt(pkg, S, d, H, P)
+    first = caches if stack else cache
+    x, long = torch.randn(S, d, device="cuda"), torch.randn(700, d, device="cuda")
+    step = lambda: model.forward_cached(x, first, pool.block_table, lens, plan, max_new=S)  # noqa: E731
+    with torch.inference_mode():
+        want = step().clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        pool2, cache2, lens2, plan2 = one_prompt(pkg, 700, d, H, P)
+        caches2 = model.new_caches(700 // P + 2, page_size=P) if stack else cache2
+        model.forward_cached(long, caches2, pool2.block_table, lens2, plan2, max_new=700)
+        others = [torch.full((1 << k,), 7, dtype=torch.uint8, device="cuda") for k in range(8, 23)]
+        for _ in range(2):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        assert all(bool((t == 7).all()) for t in others)
+        model.check_status()
+        pkg.kv_check_status()

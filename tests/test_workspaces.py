@@ -3,6 +3,7 @@
 import contextlib
 from importlib import import_module
 from types import SimpleNamespace
+from weakref import ref
 
 import pytest
 import torch
@@ -12,7 +13,7 @@ class FakeLib:
     """Answers every size with ``need`` and every other call with success."""
 
     def __init__(self):
-        self.need, self.cleared = 4096, []
+        self.need, self.cleared, self.capturing = 4096, [], False
 
     def __getattr__(self, name):
         if name.endswith("_workspace_bytes"):
@@ -27,15 +28,19 @@ def fake(pkg, monkeypatch):
     lib = FakeLib()
     monkeypatch.setattr(pkg._lib, "lib", lambda: lib)
     monkeypatch.setattr(torch.cuda, "device", lambda *a: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: lib.capturing)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: SimpleNamespace(cuda_stream=0))
     return lib
 
 
-def grow(layer, fake, need):
+def grow(module, fake, need):
     fake.need = need
-    desc = import_module(type(layer).__module__)._lib.LayerDesc()
-    layer._ensure_workspace(desc, torch.device("cpu"), stepwise=True)
-    return layer._ws
+    lib = import_module(type(module).__module__)._lib
+    if hasattr(module, "layers"):
+        module._ensure_workspace(lib.BlockDesc(), torch.device("cpu"))
+    else:
+        module._ensure_workspace(lib.LayerDesc(), torch.device("cpu"), stepwise=True)
+    return module._ws
 
 
 def test_a_replaced_workspace_takes_the_layers_graph_with_it(pkg, fake):
@@ -45,3 +50,20 @@ def test_a_replaced_workspace_takes_the_layers_graph_with_it(pkg, fake):
     assert grow(layer, fake, 4096) is first and layer._graph is graph
     assert grow(layer, fake, 1024) is first and layer._graph is graph
     assert grow(layer, fake, 8192) is not first and layer._graph is None
+
+
+@pytest.mark.parametrize("stack", [False, True])
+def test_an_outgrown_workspace_is_kept_if_a_capture_used_it(pkg, fake, stack):
+    """A caller's captured step goes on using the workspace of its capture; others are freed as before."""
+    cfg = pkg.TransformerConfig(1, 8, 32, 1, ffn_dim=64, num_layers=1, causal=True)
+    module = pkg.B200Transformer(cfg) if stack else pkg.B200TransformerLayer(32, 1)
+    held = []
+    for need, capturing in ((4096, False), (8192, False), (8192, True), (4096, False), (16384, False), (32768, True), (65536, False)):
+        fake.capturing = capturing
+        buf = grow(module, fake, need)
+        if not held or held[-1]() is not buf:
+            held.append(ref(buf))
+        del buf
+        assert module.workspace_ptr % 1024 == 0 and fake.cleared[-1] == module.workspace_ptr
+    assert [r() is not None for r in held] == [False, True, False, True, True]     # 4, 8, 16, 32, 64 KB
+    assert len(fake.cleared) == 5
