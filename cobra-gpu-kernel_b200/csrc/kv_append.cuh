@@ -71,7 +71,8 @@ __device__ __forceinline__ uint32_t kv_code4(float a, float b, float c, float d,
     // The quotient by way of the reciprocal is off by less than 2^-22 of at most
     // 127: where that could matter, within 2^-13 of a tie, it is divided. Adding
     // 1.5 2^23 rounds to a whole number, ties to even, and leaves it in the low
-    // bits; it stays in [-127, 127] since s >= max|x| / 127 but for its rounding.
+    // bits; it stays in [-127, 127] since s >= max|x| / 127 but for its rounding
+    // (of a subnormal s, to a few bits: there it is cut off).
     const float big = 12582912.0f;
     float q[4] = {a * inv, b * inv, c * inv, d * inv}, r[4];
     float off = 0.f;
@@ -85,7 +86,7 @@ __device__ __forceinline__ uint32_t kv_code4(float a, float b, float c, float d,
       if (!(s > 0.f)) return 0;
       const float x[4] = {a, b, c, d};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = __fdiv_rn(x[i], s) + big;
+      for (int i = 0; i < 4; ++i) r[i] = fminf(fmaxf(__fdiv_rn(x[i], s), -127.f), 127.f) + big;
     }
     const uint32_t lo = __byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040);
     const uint32_t hi = __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040);

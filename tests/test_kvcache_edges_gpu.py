@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import kv_reference as ref
-from tests.test_kvcache_gpu import KIND, TOL, attention_case, i32, run_attention
+from tests.test_kvcache_gpu import DTYPE, KIND, TOL, append_and_compare, attention_case, filled_cache, i32, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +113,24 @@ def test_captured_cached_step_after_a_larger_one(pkg, cuda_ok, stack):
         assert all(bool((t == 7).all()) for t in others)
         model.check_status()
         pkg.kv_check_status()
+
+
+# ---------------------------------------------------------------- append
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_append_values_near_the_least_fp32(pkg, cuda_ok, kind, dtype):
+    """A page's largest value a few times 2^-149 (the least bf16 number is 2^-133): an int8
+    scale then has few bits, and a quotient may be past 127."""
+    rng = np.random.RandomState(22)
+    P, H, dh = 16, 2, 32
+    unit = 2.0 ** -149 if dtype == "fp32" else 2.0 ** -133
+    sizes = [1, 2, 63, 64, 100, 127, 128, 150, 190, 191, 250, 317, 1000, 12345]
+    c, held = filled_cache(pkg, rng, len(sizes), H, dh, P, kind)
+    for place in (0, 5):                        # a fresh page, then more of the same in it
+        x = [np.stack([unit * np.rint(rng.uniform(-n, n, size=(H, dh))) for n in sizes for _ in range(3)]) for _ in range(2)]
+        for v in x:
+            v[::3, :, 0] = [[unit * n] * H for n in sizes]
+            v[1::3, :, 1] = [[-unit * n] * H for n in sizes]
+        t = [torch.from_numpy(v).to(DTYPE[dtype]) for v in x]
+        slots = np.array([i * P + place + k for i in range(len(sizes)) for k in range(3)], dtype=np.int64)
+        append_and_compare(pkg, c, held, t[0].cuda(), t[1].cuda(), *(v.double().numpy() for v in t), slots, kind, P)
