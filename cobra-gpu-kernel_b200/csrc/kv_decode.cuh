@@ -629,17 +629,25 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
       }
     }
   }
-  // Rows that attend to nothing: of requests without keys, and past the plan's tokens.
+  // Rows that attend to nothing: of requests without keys, and past the plan's
+  // tokens. And those that no row tile takes, of a request with more new tokens
+  // than the caller said: not-a-number, as there is nobody to tell.
   {
-    auto zero_rows = [&](int t0, int t1) {
-      const long long e1 = (long long)min(t1, a.tokens) * a.hq * a.dh;
-      for (long long i = (long long)t0 * a.hq * a.dh + lane; i < e1; i += 32) static_cast<unsigned short*>(a.out)[i] = 0;
+    const long long tok = (long long)a.hq * a.dh;
+    auto fill = [&](long long i, long long end, unsigned short x) {
+      for (i += lane; i < end; i += 32) static_cast<unsigned short*>(a.out)[i] = x;
     };
+    const int have = a.row_tiles * M;
     for (int r = w; r < a.requests; r += workers) {
-      const int c0 = a.cu_pages[r], c1 = a.cu_pages[r + 1], t0 = a.cu_new[r], t1 = a.cu_new[r + 1];
-      if (c0 == c1 && t1 > t0) zero_rows(t0, t1);
+      const int c0 = a.cu_pages[r], c1 = a.cu_pages[r + 1], t0 = a.cu_new[r], t1 = min(a.cu_new[r + 1], a.tokens);
+      if (c0 == c1) fill(t0 * tok, t1 * tok, 0);
+      else if ((long long)(t1 - t0) * a.group > have)
+        for (int i = have / a.group; i < t1 - t0; ++i)
+          for (int h = 0; h < a.c.heads; ++h)
+            fill((t0 + i) * tok + (long long)(h * a.group + max(0, have - i * a.group)) * a.dh,
+                 (t0 + i) * tok + (long long)(h + 1) * a.group * a.dh, 0x7fff);
     }
-    for (int i = a.cu_new[a.requests] + w; i < a.tokens; i += workers) zero_rows(i, i + 1);
+    for (int i = a.cu_new[a.requests] + w; i < a.tokens; i += workers) fill(i * tok, (i + 1) * tok, 0);
   }
   if (!ok) {                                      // copies in flight land before the block goes
     for (int i = used; i < issued; ++i) mbar_drain(&bars[i & 1], (i >> 1) & 1);

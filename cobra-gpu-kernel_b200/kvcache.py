@@ -331,7 +331,8 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq
     h // (query heads // cache heads). Of a request with n new tokens of
     ``seq_lens[r]`` cached ones (int32, the new ones among them), token i sees
     the keys up to its own position, or all with ``causal=False``. ``max_new``:
-    no request has more new tokens (it chooses the kernel; 1 for a decode step).
+    no request has more new tokens (it chooses the kernel; 1 for a decode step;
+    of a request that has more, rows may come out as not-a-number).
     ``scale`` is head_dim ** -0.5 if not given. A row that sees no key is 0, and
     so are rows past the plan's tokens. Returns ``out``, contiguous, q's dtype.
     """

@@ -370,7 +370,8 @@ B200L_API int b200l_kv_read(const b200l_kv_cache* cache, const int64_t* slots, i
  * with causal those up to its own position seq_lens[r] - n + i. Query head h
  * reads key/value head h / (num_heads / cache heads). A row that sees no key is
  * 0, as are the rows from cu_new[requests] on. Keys behind block table entries
- * outside the cache are not there. */
+ * outside the cache are not there. A request with more than max_new new tokens
+ * has not-a-number in the rows that the kernel chosen by max_new does not take. */
 typedef struct b200l_kv_attn_desc {
     const void* q;              /* [tokens, num_heads, head_dim], dims contiguous */
     void* out;                  /* the same shape, contiguous */

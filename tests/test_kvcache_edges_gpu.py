@@ -55,6 +55,29 @@ def test_attention_counts_keys_of_small_values(pkg, cuda_ok, kind, dtype, hq, hk
             assert (err <= bound).all(), f"{lens} {new} {spread}: {(err / np.abs(want).clip(1e-30)).max():.3g} of the output"
 
 
+# ---------------------------------------------------------------- calls at odds with their lengths
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,dh", [(2, 2, 64), (6, 2, 32), (8, 1, 128), (6, 2, 256), (80, 2, 64), (3, 3, 33)])
+def test_attention_with_more_new_tokens_than_said(pkg, cuda_ok, hq, hkv, dh, dtype):
+    """A max_new below the truth: every row is either right or not-a-number, those within it
+    are right, and the other requests' too."""
+    group = hq // hkv
+    s = attention_case(pkg, 23 + dh, "int8", dtype, hq, hkv, dh, 16, [5, 90, 0, 400, 7, 0], [1, 61, 0, 9, 1, 3])
+    want, vmax = ref.attention(s["q"].double().numpy(), s["kc"], s["vc"], s["ks"], s["vs"], s["kind"], s["table"],
+                               s["lens"], s["cu"], True, dh ** -0.5)
+    plan = pkg.KVPlan(i32(s["cu"]), i32(s["cup"]), None, None, None)
+    first = np.concatenate([np.arange(n) for n in s["new"]])      # each row's place in its request
+    for said in (0, 1, 2, 5, 40):
+        out = torch.full_like(s["q"], 7.0).cuda()
+        pkg.kv_attention(s["q"].cuda(), s["c"], i32(s["table"]), i32(s["lens"]), plan, max_new=said, out=out)
+        pkg.kv_check_status()
+        got = out.double().cpu().numpy()
+        lost = np.isnan(got).all(-1)
+        assert not lost[first < said].any() and not lost[-3:].any()
+        assert lost.any() == (61 * group > 32 and said * group <= 32)
+        assert (lost | (np.abs(got - want) <= TOL[dtype] * vmax).all(-1)).all()
+
+
 # ---------------------------------------------------------------- workspaces of cached steps
 def one_prompt(pkg, S, d, H, P=16):
     """Pool, cache, lengths and plan of one request's first S tokens."""
