@@ -28,7 +28,7 @@ EXPORTED = (
 # Element types of b200l_convert.
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 # Codes of the paged key/value cache.
 KV_INT8, KV_E4M3 = 0, 1
@@ -94,7 +94,7 @@ class KVPlanDesc(ctypes.Structure):
     _fields_ = [
         ("old_lens", c_void_p), ("new_lens", c_void_p), ("block_table", c_void_p), ("table_stride", c_int64),
         ("free_pages", c_void_p), ("free_count", c_void_p), ("cu_new", c_void_p), ("cu_pages", c_void_p),
-        ("positions", c_void_p), ("slots", c_void_p), ("info", c_void_p),
+        ("positions", c_void_p), ("slots", c_void_p), ("info", c_void_p), ("unplaced", c_void_p),
         ("requests", c_int32), ("table_width", c_int32), ("page_size", c_int32), ("capacity", c_int32),
         ("max_tokens", c_int32),
     ]

@@ -76,6 +76,7 @@ int kv_plan_run(const b200l_kv_plan_desc* d, cudaStream_t st) {
   a.positions = d->positions;
   a.slots = reinterpret_cast<long long*>(d->slots);
   a.info = d->info;
+  a.unplaced = d->unplaced;
   a.requests = d->requests;
   a.width = d->table_width;
   a.page = d->page_size;

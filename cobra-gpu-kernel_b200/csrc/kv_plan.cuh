@@ -39,6 +39,7 @@ struct KvPlanArgs {
   int* positions;
   long long* slots;
   int* info;             // free pages after the step, pages that were missing
+  int* unplaced;         // new tokens past max_tokens, or NULL
   int requests, width, page, log2_page, capacity, max_tokens;
 };
 
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(KvPlanArgs a) {
   if (first && threadIdx.x == 0) {
     a.info[0] = max(top - take, 0);
     a.info[1] = clip(max(take - top, 0) + (long long)s_over);
+    if (a.unplaced) *a.unplaced = max(total - a.max_tokens, 0);
   }
 
   // Page at height i of the stack with the pages given back on top of it.

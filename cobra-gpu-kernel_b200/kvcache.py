@@ -48,6 +48,7 @@ class KVPlan(NamedTuple):
     positions: torch.Tensor   # int32 [max_tokens]: each new token's position, -1 past the last
     slots: torch.Tensor       # int64 [max_tokens]: page * page_size + place, -1 for none
     info: torch.Tensor        # int32 [2]: free pages left, pages that were missing
+    unplaced: Optional[torch.Tensor] = None   # int32 [1]: new tokens past max_tokens
 
 
 def padded_head_dim(head_dim: int) -> int:
@@ -127,7 +128,7 @@ def _refuse_cache(cache: KVCache, head_dim: int, index: int) -> None:
 # Descriptors as the library reads them (the layouts of ``_lib.KVCacheDesc``,
 # ``KVPlanDesc``, ``KVRows`` and ``KVAttnDesc``), packed in one step.
 _pack_cache = struct.Struct("@PPPPqiiii").pack
-_pack_plan = struct.Struct("@PPPqPPPPPPPiiiii4x").pack
+_pack_plan = struct.Struct("@PPPqPPPPPPPPiiiii4x").pack
 _pack_rows = struct.Struct("@PPqqqqqqi4x").pack
 _pack_attn = struct.Struct("@PPqqPqPPPiiiiiiif").pack
 
@@ -214,7 +215,9 @@ def kv_plan(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.T
     write, so a repeated call gives the same answer. The step is adopted by going
     on from ``new_lens`` and ``info[0]``. Where ``info[1]`` pages were missing,
     their table entries and slots are -1: plan again with other ``new_lens``.
-    ``max_tokens`` bounds the new tokens; entries past them are -1.
+    ``max_tokens`` bounds the new tokens; entries past them are -1. ``unplaced``
+    tokens that it left out have no slot although the lengths count them: not to be
+    adopted either, for attention would read what their places held before.
     """
     index = _cuda(old_lens, "old_lens")
     R = old_lens.numel()
@@ -241,20 +244,21 @@ def kv_plan(old_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.T
 def _plan(stream, old_lens, new_lens, table, stride, free_pages, free_count, page_size, max_tokens) -> KVPlan:
     R, width = table.shape
     # One allocation: slots (8 bytes each), then the int32 outputs.
-    buf = old_lens.new_empty(3 * max_tokens + 2 * R + 4)
+    buf = old_lens.new_empty(3 * max_tokens + 2 * R + 5)
     at = buf.data_ptr()
-    slots, positions, cu_new, cu_pages, info = torch.unsafe_split_with_sizes(
-        buf, (2 * max_tokens, max_tokens, R + 1, R + 1, 2))
+    slots, positions, cu_new, cu_pages, info, unplaced = torch.unsafe_split_with_sizes(
+        buf, (2 * max_tokens, max_tokens, R + 1, R + 1, 2, 1))
     p_pos = at + 8 * max_tokens
     p_new = p_pos + 4 * max_tokens
     p_pages = p_new + 4 * (R + 1)
+    p_info = p_pages + 4 * (R + 1)
     rc = _lib.lib().b200l_kv_plan(
         _pack_plan(old_lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(), stride, free_pages.data_ptr(),
-                   free_count.data_ptr(), p_new, p_pages, p_pos, at, p_pages + 4 * (R + 1), R, width, page_size,
+                   free_count.data_ptr(), p_new, p_pages, p_pos, at, p_info, p_info + 8, R, width, page_size,
                    free_pages.numel(), max_tokens), stream)
     if rc:
         _lib.check(rc)
-    return KVPlan(cu_new, cu_pages, positions, slots.view(torch.int64), info)
+    return KVPlan(cu_new, cu_pages, positions, slots.view(torch.int64), info, unplaced)
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: KVCache) -> None:
@@ -418,7 +422,7 @@ class KVPool:
                        max_tokens=max_tokens)
 
     def adopt(self, new_lens: torch.Tensor, plan: KVPlan) -> None:
-        """Goes on from the lengths and free pages of a plan that missed no pages."""
+        """Goes on from the lengths and free pages of a plan that missed no pages and placed every token."""
         self.lens.copy_(new_lens)
         self.free_count.copy_(plan.info[:1])
 

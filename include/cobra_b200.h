@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define B200L_ABI_VERSION 5
+#define B200L_ABI_VERSION 6
 
 enum b200l_status {
     B200L_OK = 0,
@@ -320,7 +320,9 @@ typedef struct b200l_kv_cache {
  * is not written, so a call repeated gives the same answer; the caller adopts
  * new_lens and info[0] to go on. With info[1] > 0 pages were missing: their
  * table entries and slots are -1, and the caller plans again with other
- * new_lens instead of adopting. */
+ * new_lens instead of adopting. So it does with *unplaced > 0: that many new
+ * tokens are counted in the lengths but have no slot, and what attends to their
+ * places reads what the pages held before. */
 typedef struct b200l_kv_plan_desc {
     const int32_t* old_lens;    /* [requests] */
     const int32_t* new_lens;    /* [requests] */
@@ -333,6 +335,7 @@ typedef struct b200l_kv_plan_desc {
     int32_t* positions;         /* out [max_tokens]: position in its request; -1 past the last new token */
     int64_t* slots;             /* out [max_tokens]: slot; -1 past the last new token */
     int32_t* info;              /* out [2]: free pages left, pages missing */
+    int32_t* unplaced;          /* out [1], may be NULL: new tokens past max_tokens */
     int32_t requests;           /* 1 .. B200L_KV_MAX_REQUESTS */
     int32_t table_width;
     int32_t page_size;

@@ -56,6 +56,19 @@ def test_attention_counts_keys_of_small_values(pkg, cuda_ok, kind, dtype, hq, hk
 
 
 # ---------------------------------------------------------------- calls at odds with their lengths
+@pytest.mark.parametrize("R", [3, 700])
+def test_plan_says_how_many_tokens_have_no_slot(pkg, cuda_ok, R):
+    P, width = 16, 4
+    rng = np.random.RandomState(R)
+    new = [int(n) for n in rng.randint(0, width * P + 1, size=R)]
+    total = sum(new)
+    free = torch.arange(R * width, dtype=torch.int32, device="cuda")
+    for most in (0, 1, total - 1, total, total + 3):
+        plan = pkg.kv_plan(i32([0] * R), i32(new), i32([[-1] * width] * R), free, i32([R * width]), page_size=P, max_tokens=most)
+        assert plan.unplaced.tolist() == [max(total - most, 0)]
+        assert plan.cu_new[-1].item() == total and int((plan.slots >= 0).sum()) == min(most, total)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("hq,hkv,dh", [(2, 2, 64), (6, 2, 32), (8, 1, 128), (6, 2, 256), (80, 2, 64), (3, 3, 33)])
 def test_attention_with_more_new_tokens_than_said(pkg, cuda_ok, hq, hkv, dh, dtype):
