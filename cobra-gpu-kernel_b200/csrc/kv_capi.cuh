@@ -134,11 +134,11 @@ int kv_append_run(const b200l_kv_cache* cache, const b200l_kv_rows* rows, const 
   KvAppendArgs a;
   int rc = kv_check_cache(cache, &a.c);
   if (rc) return rc;
-  if (!rows || !rows->k || !rows->v) return fail(B200L_ERR_NULL_POINTER, "kv_append: k or v is NULL");
+  if (!rows) return fail(B200L_ERR_NULL_POINTER, "kv_append: rows descriptor is NULL");
   if (tokens < 0 || tokens > (1ll << 30)) return fail(B200L_ERR_BAD_SHAPE, "kv_append: %lld tokens", (long long)tokens);
   if (rows->dtype < 0 || rows->dtype > 2)
     return fail(B200L_ERR_BAD_SHAPE, "kv_append: dtype must be B200L_DTYPE_F32 / _F16 / _BF16");
-  if (tokens && !slots) return fail(B200L_ERR_NULL_POINTER, "kv_append: slots is NULL");
+  if (tokens && (!rows->k || !rows->v || !slots)) return fail(B200L_ERR_NULL_POINTER, "kv_append: k, v or slots is NULL");
   DevInfo dev;
   if ((rc = device_info(&dev))) return rc;
   if (tokens == 0) return B200L_OK;

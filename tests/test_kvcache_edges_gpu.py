@@ -152,6 +152,21 @@ def test_captured_cached_step_after_a_larger_one(pkg, cuda_ok, stack):
 
 
 # ---------------------------------------------------------------- append
+def test_a_step_of_no_tokens(pkg, cuda_ok):
+    """Every request idle: plan, append, read and attention take no tokens, and the cache stays."""
+    c, held = filled_cache(pkg, np.random.RandomState(24), 6, 2, 64, 16, "int8")
+    table, lens = i32([[0, 1], [2, -1]]), i32([20, 7])
+    plan = pkg.kv_plan(lens, lens, table, i32([3, 4, 5]), i32([3]), page_size=16, max_tokens=0)
+    assert plan.cu_new.tolist() == [0, 0, 0] and plan.slots.shape == (0,) and plan.info.tolist() == [3, 0]
+    for dtype in DTYPE.values():
+        x = torch.empty(0, 2, 64, dtype=dtype, device="cuda")
+        pkg.kv_append(x, x, plan.slots, c)
+    assert all(t.shape == (0, 2, 64) for t in pkg.kv_read(plan.slots, c, 64))
+    assert pkg.kv_attention(x.half(), c, table, lens, plan, max_new=0).shape == (0, 2, 64)
+    for t, h in zip((c.k, c.k_scale, c.v, c.v_scale), held):
+        assert np.array_equal(t.view(torch.uint8).cpu().numpy() if t.dtype == torch.int8 else t.cpu().numpy(), h)
+
+
 @pytest.mark.parametrize("kind", ["int8", "fp8"])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_append_values_near_the_least_fp32(pkg, cuda_ok, kind, dtype):
