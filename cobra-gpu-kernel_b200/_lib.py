@@ -20,7 +20,7 @@ EXPORTED = (
     "b200l_outproj_res_ln", "b200l_layer_forward_noalloc", "b200l_block_workspace_bytes",
     "b200l_block_forward", "b200l_row_layernorm", "b200l_cast_f16",
     "b200l_kernel_workspace_bytes", "b200l_debug_arm", "b200l_noalloc_read_status",
-    "b200l_convert",
+    "b200l_convert", "b200l_exchange_capture_mode",
     "b200l_block_finish", "b200l_kv_plan", "b200l_kv_append", "b200l_kv_read",
     "b200l_kv_attention_workspace_bytes", "b200l_kv_attention",
 )
@@ -29,6 +29,9 @@ EXPORTED = (
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
 ABI_VERSION = 6
+
+# b200l_exchange_capture_mode.
+CAPTURE_RELAXED = 2
 
 # Codes of the paged key/value cache.
 KV_INT8, KV_E4M3 = 0, 1
@@ -153,6 +156,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200l_kernel_workspace_bytes": (c_size_t, [P]),
         "b200l_debug_arm": (c_int, [P, c_int32, ctypes.c_uint64, P]),
         "b200l_noalloc_read_status": (c_int, [P]),
+        "b200l_exchange_capture_mode": (c_int, [P]),
         "b200l_convert": (c_int, [P, c_int32, P, c_int32, ctypes.c_int64, P]),
         "b200l_kv_plan": (c_int, [P, P]),
         "b200l_kv_append": (c_int, [P, P, P, c_int64, P]),

@@ -708,6 +708,15 @@ int b200l_clear_status(void* workspace, void* stream) {
   return B200L_OK;
 }
 
+int b200l_exchange_capture_mode(int32_t* mode) {
+  if (!mode) return fail(B200L_ERR_NULL_POINTER, "mode is NULL");
+  cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(*mode);
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&m);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
+  *mode = static_cast<int32_t>(m);
+  return B200L_OK;
+}
+
 int b200l_debug_arm(void* workspace, int32_t site, uint64_t wait_limit_ns, void* stream) {
   if (!workspace) return fail(B200L_ERR_NULL_POINTER, "workspace is NULL");
   if (site < 0 || site > kSiteGemmOperand) return fail(B200L_ERR_BAD_SHAPE, "unknown fault site %d", site);

@@ -24,6 +24,7 @@ from typing import Dict, NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
+from .workspace import new_workspace
 
 PAGE_SIZES = (16, 32, 64, 128)
 _KINDS = {torch.int8: _lib.KV_INT8, torch.float8_e4m3fn: _lib.KV_E4M3}
@@ -153,31 +154,27 @@ class _Workspace:
     """A workspace of each (device, stream): calls on one stream run one after
     another, so they can share it. (Graphs captured on one stream share it too and
     are not to be replayed at the same time.) A buffer that was outgrown is kept (a
-    captured graph may still use it); each is at least twice the one before. One
-    that was made during a capture has its status block cleared by every call: the
-    clearing that made it usable is in that graph, not in the stream."""
+    captured graph may still use it); each is at least twice the one before."""
 
     def __init__(self) -> None:
         self._held: Dict[Tuple[int, int], list] = {}
 
-    def get(self, index: int, stream: int) -> Tuple[int, int, bool]:
-        """(address, bytes, to be cleared), 0 bytes if there is none yet."""
+    def get(self, index: int, stream: int) -> Tuple[int, int]:
+        """(address, bytes), 0 bytes if there is none yet."""
         held = self._held.get((index, stream))
-        return held[-1][:3] if held else (0, 0, False)
+        return held[-1][:2] if held else (0, 0)
 
     def grow(self, index: int, stream: int, need: int) -> Tuple[int, int]:
         held = self._held.setdefault((index, stream), [])
         size = max(need, 2 * held[-1][1] if held else 0)
-        buf = torch.empty(size + 1024, dtype=torch.uint8, device=torch.device("cuda", index))
-        ptr = (buf.data_ptr() + 1023) // 1024 * 1024
-        _lib.check(_lib.lib().b200l_clear_status(ptr, stream))
-        held.append((ptr, size, torch.cuda.is_current_stream_capturing(), buf))
-        return ptr, size
+        buf, off = new_workspace(size, torch.device("cuda", index))
+        held.append((buf.data_ptr() + off, size, buf))
+        return held[-1][:2]
 
     def check(self) -> None:
         for (index, stream), held in self._held.items():
             with torch.cuda.device(index):
-                for ptr, _, _, _ in held:
+                for ptr, _, _ in held:
                     rc = _lib.lib().b200l_read_status(ptr, stream)
                     if rc:
                         message = _lib.last_error()
@@ -381,9 +378,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq
 
 def _attention(stream, index, c, desc) -> None:
     L = _lib.lib()
-    ws, size, clear = _workspace.get(index, stream)
-    if clear:
-        _lib.check(L.b200l_clear_status(ws, stream))
+    ws, size = _workspace.get(index, stream)
     rc = L.b200l_kv_attention(c, desc, ws, size, stream)
     if rc == _lib.ERR_WORKSPACE:
         need = L.b200l_kv_attention_workspace_bytes(c, desc)

@@ -127,6 +127,12 @@ B200L_API size_t b200l_kernel_workspace_bytes(const b200l_layer_desc* desc);
 /* Zeroes the status word at the start of a workspace (async on stream). */
 B200L_API int b200l_clear_status(void* workspace, void* stream);
 
+/* cudaThreadExchangeStreamCaptureMode: swaps the calling thread's mode with *mode.
+ * In B200L_CAPTURE_RELAXED a thread may allocate and synchronise on other streams
+ * while one is captured: how a workspace is made and cleared outside the graph. */
+#define B200L_CAPTURE_RELAXED 2
+B200L_API int b200l_exchange_capture_mode(int32_t* mode);
+
 /* Reads the status word (synchronises ``stream``): 0 when no kernel recorded a
  * failure, else the B200L_ERR_* code that was recorded. */
 B200L_API int b200l_read_status(const void* workspace, void* stream);

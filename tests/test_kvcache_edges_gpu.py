@@ -1,5 +1,7 @@
 """The paged 8-bit cache on a B200 where a step's numbers lie apart or its calls are at odds."""
 
+from importlib import import_module
+
 import numpy as np
 import pytest
 import torch
@@ -185,3 +187,78 @@ def test_append_values_near_the_least_fp32(pkg, cuda_ok, kind, dtype):
         t = [torch.from_numpy(v).to(DTYPE[dtype]) for v in x]
         slots = np.array([i * P + place + k for i in range(len(sizes)) for k in range(3)], dtype=np.int64)
         append_and_compare(pkg, c, held, t[0].cuda(), t[1].cuda(), *(v.double().numpy() for v in t), slots, kind, P)
+
+
+def test_a_recorded_failure_stays_until_it_is_read(pkg, cuda_ok):
+    """In a workspace that a capture made: neither a later call on its stream nor a replay erases
+    what an earlier call recorded, and it is no memory that the graph uses otherwise."""
+    s = attention_case(pkg, 25, "int8", "fp16", 4, 2, 64, 16, [90, 3000, 7], [1, 1, 1])
+    plan = pkg.KVPlan(i32(s["cu"]), i32(s["cup"]), None, None, None)
+    q, table, lens = s["q"].cuda(), i32(s["table"]), i32(s["lens"])
+    call = lambda: pkg.kv_attention(q, s["c"], table, lens, plan, max_new=1)  # noqa: E731
+    want = call()
+    pkg.kv_check_status()
+    held = import_module(pkg.__name__ + ".kvcache")._workspace._held
+    side = next(st for st in (torch.cuda.Stream() for _ in range(64)) if (0, st.cuda_stream) not in held)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        temp = torch.empty(1 << 26, dtype=torch.uint8, device="cuda").fill_(0xff)
+        span = (temp.data_ptr(), temp.data_ptr() + temp.numel())
+        del temp
+        call()                                  # as one layer's step and the next one's
+        out = call()
+    ptr, buf = held[0, side.cuda_stream][-1][0], held[0, side.cuda_stream][-1][-1]
+    assert not span[0] <= ptr < span[1]
+    code = buf[ptr - buf.data_ptr():][:4].view(torch.int32)
+
+    def eager():
+        with torch.cuda.stream(side):
+            return call()
+
+    for _ in range(2):
+        for go in (lambda: (graph.replay(), out)[1], eager):
+            got = go()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            pkg.kv_check_status()
+            code.fill_(-7)
+            torch.cuda.synchronize()
+            go()
+            torch.cuda.synchronize()
+            with pytest.raises(pkg._lib.B200LError, match="TIMEOUT"):
+                pkg.kv_check_status()
+
+
+@pytest.mark.parametrize("stack", [False, True])
+def test_workspace_made_by_a_capture(pkg, cuda_ok, stack):
+    """A captured cached step that needs a larger workspace than there was: right at each replay,
+    in a second graph replayed before it, and its status block clear from the start."""
+    d, H, S, P = 128, 4, 50, 16
+    torch.manual_seed(6)
+    if stack:
+        model = pkg.B200Transformer(pkg.TransformerConfig(1, 8, d, H, ffn_dim=256, num_layers=2, causal=True)).cuda().eval()
+        small, caches = model.new_caches(2, page_size=P), model.new_caches(S // P + 2, page_size=P)
+    else:
+        model = pkg.B200TransformerLayer(d, H, True).cuda().eval()
+        small, caches = (pkg.new_kv_cache(n, H, d // H, page_size=P) for n in (2, S // P + 2))
+    x = torch.randn(S, d, device="cuda")
+    with torch.inference_mode():
+        pool, _, lens, plan = one_prompt(pkg, 3, d, H, P)
+        model.forward_cached(x[:3], small, pool.block_table, lens, plan, max_new=3)       # packs the weights
+        before = model.workspace_ptr
+        pool, _, lens, plan = one_prompt(pkg, S, d, H, P)
+        graphs, outs = [], []
+        for _ in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                outs.append(model.forward_cached(x, caches, pool.block_table, lens, plan, max_new=S))
+        assert model.workspace_ptr != before
+        model.check_status()
+        for i in (1, 0, 1):
+            outs[i].zero_()
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        model.check_status()
+        pkg.kv_check_status()
+        want = model.forward_cached(x, caches, pool.block_table, lens, plan, max_new=S)
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want) and want.any()

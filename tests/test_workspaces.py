@@ -13,7 +13,13 @@ class FakeLib:
     """Answers every size with ``need`` and every other call with success."""
 
     def __init__(self):
-        self.need, self.cleared, self.capturing = 4096, [], False
+        self.need, self.cleared, self.capturing, self.aside = 4096, [], False, False
+
+    @contextlib.contextmanager
+    def on_another_stream(self, stream):
+        self.aside = True
+        yield
+        self.aside = False
 
     def __getattr__(self, name):
         if name.endswith("_workspace_bytes"):
@@ -28,7 +34,9 @@ def fake(pkg, monkeypatch):
     lib = FakeLib()
     monkeypatch.setattr(pkg._lib, "lib", lambda: lib)
     monkeypatch.setattr(torch.cuda, "device", lambda *a: contextlib.nullcontext())
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: lib.capturing)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: lib.capturing and not lib.aside)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda *a: SimpleNamespace(cuda_stream=99, synchronize=lambda: None))
+    monkeypatch.setattr(torch.cuda, "stream", lib.on_another_stream)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: SimpleNamespace(cuda_stream=0))
     return lib
 
