@@ -19,6 +19,7 @@ current stream of their tensors' device through the sm_100a library
 from __future__ import annotations
 
 import struct
+import threading
 from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
@@ -154,10 +155,17 @@ class _Workspace:
     """A workspace of each (device, stream): calls on one stream run one after
     another, so they can share it. (Graphs captured on one stream share it too and
     are not to be replayed at the same time.) A buffer that was outgrown is kept (a
-    captured graph may still use it); each is at least twice the one before."""
+    captured graph may still use it); each is at least twice the one before. A call is
+    several launches that hand one another numbers in it, so threads take turns."""
 
     def __init__(self) -> None:
         self._held: Dict[Tuple[int, int], list] = {}
+        self._turns: Dict[Tuple[int, int], threading.Lock] = {}
+
+    def turn(self, index: int, stream: int) -> threading.Lock:
+        """To be held from the choice of the buffer to the call's last launch."""
+        key = (index, stream)
+        return self._turns.get(key) or self._turns.setdefault(key, threading.Lock())
 
     def get(self, index: int, stream: int) -> Tuple[int, int]:
         """(address, bytes), 0 bytes if there is none yet."""
@@ -172,9 +180,9 @@ class _Workspace:
         return held[-1][:2]
 
     def check(self) -> None:
-        for (index, stream), held in self._held.items():
+        for (index, stream), held in list(self._held.items()):
             with torch.cuda.device(index):
-                for ptr, _, _ in held:
+                for ptr, _, _ in list(held):
                     rc = _lib.lib().b200l_read_status(ptr, stream)
                     if rc:
                         message = _lib.last_error()
@@ -378,12 +386,13 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq
 
 def _attention(stream, index, c, desc) -> None:
     L = _lib.lib()
-    ws, size = _workspace.get(index, stream)
-    rc = L.b200l_kv_attention(c, desc, ws, size, stream)
-    if rc == _lib.ERR_WORKSPACE:
-        need = L.b200l_kv_attention_workspace_bytes(c, desc)
-        ws, size = _workspace.grow(index, stream, need)
+    with _workspace.turn(index, stream):
+        ws, size = _workspace.get(index, stream)
         rc = L.b200l_kv_attention(c, desc, ws, size, stream)
+        if rc == _lib.ERR_WORKSPACE:
+            need = L.b200l_kv_attention_workspace_bytes(c, desc)
+            ws, size = _workspace.grow(index, stream, need)
+            rc = L.b200l_kv_attention(c, desc, ws, size, stream)
     if rc:
         _lib.check(rc)
 

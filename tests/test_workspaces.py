@@ -1,6 +1,8 @@
 """CPU tests of who holds workspaces: the library's sizes and clears are made up, memory is the host's."""
 
 import contextlib
+import threading
+import time
 from importlib import import_module
 from types import SimpleNamespace
 from weakref import ref
@@ -75,3 +77,46 @@ def test_an_outgrown_workspace_is_kept_if_a_capture_used_it(pkg, fake, stack):
         assert module.workspace_ptr % 1024 == 0 and fake.cleared[-1] == module.workspace_ptr
     assert [r() is not None for r in held] == [False, True, False, True, True]     # 4, 8, 16, 32, 64 KB
     assert len(fake.cleared) == 5
+
+
+def test_threads_take_turns_at_a_streams_workspace(pkg, monkeypatch):
+    """A call's launches pass numbers through the workspace: no other thread's call on the
+    same stream comes between them, nor between the choice of a buffer and its use; calls
+    on different streams do not wait for one another."""
+    kv = import_module(pkg.__name__ + ".kvcache")
+    inside, most, made = {}, {}, []
+    meet = threading.Barrier(2)
+
+    class Lib:
+        def b200l_kv_attention(self, c, desc, ws, size, stream):
+            if stream != 5:
+                meet.wait(10)               # both streams' calls at once, or the barrier breaks
+            inside[stream] = inside.get(stream, 0) + 1
+            most[stream] = max(most.get(stream, 0), inside[stream])
+            time.sleep(0.01)
+            inside[stream] -= 1
+            return 0 if size else -4
+
+        def b200l_kv_attention_workspace_bytes(self, c, desc):
+            return 4096
+
+    lib = Lib()
+    monkeypatch.setattr(pkg._lib, "lib", lambda: lib)
+    held = kv._Workspace()
+    held.grow = lambda index, stream, need: made.append(stream) or held._held.setdefault((index, stream), [(1024, need, None)])[-1][:2]
+    monkeypatch.setattr(kv, "_workspace", held)
+    bad = []
+
+    def run(stream):
+        try:
+            kv._attention(stream, 0, b"", b"")
+        except Exception as e:              # (a thread's exception is seen below)
+            bad.append(e)
+
+    for streams in ([5] * 8, [6, 7]):
+        threads = [threading.Thread(target=run, args=(s,)) for s in streams]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(30)
+    assert not bad and most == {5: 1, 6: 1, 7: 1} and sorted(made) == [5, 6, 7]
