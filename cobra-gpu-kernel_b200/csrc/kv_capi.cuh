@@ -255,8 +255,13 @@ int kv_attn_plan(const b200l_kv_cache* cache, const b200l_kv_attn_desc* d, KvAtt
   const int rows = (d->max_new < d->tokens ? d->max_new : d->tokens) * a.group;
   DevInfo dev;
   if ((rc = device_info(&dev))) return rc;
-  // A request's rows fit one or two 16-row tiles of mma.sync, whose kernel is
-  // bound by HBM; beyond, tcgen05's 128-row tiles.
+  // A request's rows fit one or two tiles of mma.sync, whose kernel is bound by
+  // HBM; beyond, tcgen05's 128-row tiles. Both at 33 to 64 rows (8 key heads, int8, us,
+  // the few-row kernel in several row tiles first): one request of 30000 tokens
+  // 61-68 against 43-44 at head_dim 64, 138-143 against 56-57 at 128, 144-160 against
+  // 94-95 at 256; 64 requests of 4000 219-230 against 247-255, 357-372 against
+  // 348-352, 654-863 against 564-571. (At 32 rows the few-row kernel takes 80, 178 and
+  // 145 on the one long request, 133, 213 and 451 on the 64.)
   p->prompt = rows > 32;
   if (p->prompt) {
     const int mq = p->dhp == 256 ? 128 : 256;

@@ -12,7 +12,7 @@
 // contribution, and no accumulator is rescaled per page. Sums and maxima are
 // fp32; fp16 rounds q (scaled by a power of two to [1, 2) at the row's largest
 // if it comes as bf16: exact but for what is 2^-14 of it) and the weights of the
-// numerator: to 2^-12 of themselves, below 2^-14 to 2^-25 of the largest
+// numerator: to 2^-11 of themselves, below 2^-14 to 2^-25 of the largest
 // contribution. The denominator must not lose those, for there a key counts with
 // 2^t whatever its values' size: it sums the weights in fp32.
 //
@@ -29,9 +29,9 @@
 // leave a piece adding them itself, 8 us). Where tables are too narrow for it to
 // be worth it, stretches are whole pairs and there is nothing to join.
 //
-// Measured: 256 requests of about 7000 tokens, 32 / 8 heads of 128, int8 585-654 us
-// (3.7 GB, 88-98 % of HBM's rate); 2 requests of 100000, 16 heads of 64, e4m3 82-86 us
-// (74-77 %); 64 ragged requests, 32 / 8 heads of 128 106-108 us (75 %): the rest is the
+// Measured: 256 requests of about 7000 tokens, 32 / 8 heads of 128, int8 594-666 us
+// (3.7 GB, 86-97 % of HBM's rate); 2 requests of 100000, 16 heads of 64, e4m3 82-83 us
+// (77 %); 64 ragged requests, 32 / 8 heads of 128 104-108 us (75-77 %): the rest is the
 // first loads' latency, the join, and warps that end apart.
 //
 // Products are mma.sync m16n8k16: one tile of M rows has too little work for
@@ -81,7 +81,13 @@ struct KvDecCfg {
   static constexpr int M = 8 * NR;
   static constexpr int QB = QSM ? M * DHP * 2 : 0;
   static constexpr int SMEM = WARPS * (SLOTS * 2 * CODE + QB) + WARPS * SLOTS * 8 + WARPS * SLOTS * 4 * 8 + 64 + 1024;
-  static constexpr int CTAS = DHP * NR >= 512 || NR == 4 ? 2 : 3;     // resident per SM (registers)
+  // Blocks of an SM: three of 168 registers, two of 255 where accumulators and Q need
+  // them. At DHP NR = 256 three spill 360 bytes (head_dim 256, 8 rows) or 600 (128, 16
+  // rows); there two, which do not spill, measured less: 32 requests of 2000 tokens, 8
+  // heads, int8, 63 against 77 us and 48 against 66; guesses of 1-5 tokens, 4 heads of
+  // 256, 46 against 60. Up to DHP NR = 128 the spills are 0 to 48 bytes; 32 rows spill
+  // up to 460 with 255.
+  static constexpr int CTAS = DHP * NR >= 512 || NR == 4 ? 2 : 3;
 };
 
 // A warp's stretch of the keys of all (request, head, row tile) triples, in
@@ -468,7 +474,8 @@ __global__ void __launch_bounds__(128, KvDecCfg<DHP, NR>::CTAS)
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
         const float2 sc = scl[s * 4 + min((16 * j) >> lb, nbox - 1)];
-        // A scale of 0 (a page of zeros) has no logarithm: 2^-100 stands for it.
+        // A scale of 0 (a page of zeros) has no logarithm: 2^-100 stands for it, and
+        // for any that is less.
         const float sv = fmaxf(sc.y, 7.8886090522101181e-31f);
         const float lv = sc.y == sc.y ? lg2_approx(sv) : sc.y;
         inv[j] = sv < INFINITY ? rcp_approx(sv) : 0.f;

@@ -17,7 +17,9 @@
 // products: per 16 keys, one page's worth at least, the softmax has c = scale
 // log2(e) s_k, log2 s_v and 1 / s_v, so that u = c s + log2 s_v is the one fused
 // multiply-add that the exponent needs anyway, the row maximum is taken per 16
-// raw scores (c >= 0) and the row sum is corrected once per 16 weights.
+// raw scores (c >= 0) and the row sum is corrected once per 16 weights. The sum is
+// of the fp32 weights; P has them as fp16, off by 2^-11 of themselves or, below
+// 2^-14, by 2^-25 of the largest contribution.
 //
 // Warps: 0 loads pages and scales, 1 issues S of both tiles, 2 / 3 issue P V of
 // tile 0 / 1, 4-7 convert, 8.. are the softmax: eight per tile, 16 rows a warp,
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DHP>::THREADS, 1) kv_prompt_kernel
             // become not-a-number, and their visible scores with them; its constants are
             // finite.
             const bool fine = sk - sk == 0.f && sv - sv == 0.f;
-            const float svc = fmaxf(sv, 7.8886090522101181e-31f);      // 2^-100 for a page of zeros
+            const float svc = fmaxf(sv, 7.8886090522101181e-31f);      // 2^-100 for a page of zeros, or less
             float4 c;
             c.x = fine ? sk : 0.f;
             c.y = !there ? -INFINITY : fine ? lg2_approx(svc) : 0.f;

@@ -307,8 +307,8 @@ def _append(stream, c, rows, slots, T) -> None:
 def kv_read(slots: torch.Tensor, cache: KVCache, head_dim: int, *,
             dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that the codes of ``slots`` (int64 ``[n]``) stand for,
-    ``[n, heads, head_dim]`` each, rounded once to ``dtype``; slots outside the
-    cache read as 0."""
+    ``[n, heads, head_dim]`` each, code times scale in fp32, rounded to ``dtype``;
+    slots outside the cache read as 0."""
     index = _cuda(slots, "slots")
     code = _DTYPES.get(dtype)
     if code is None or slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
@@ -344,6 +344,10 @@ def kv_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, seq
     of a request that has more, rows may come out as not-a-number).
     ``scale`` is head_dim ** -0.5 if not given. A row that sees no key is 0, and
     so are rows past the plan's tokens. Returns ``out``, contiguous, q's dtype.
+
+    Calls on one stream share a workspace, and so do graphs captured on one stream
+    (``torch.cuda.graph`` captures all on the same one unless it is given another):
+    such graphs must not be replayed at the same time.
     """
     index = _cuda(q, "q")
     if q.dim() != 3:

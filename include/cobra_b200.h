@@ -368,7 +368,7 @@ typedef struct b200l_kv_rows {
 B200L_API int b200l_kv_append(const b200l_kv_cache* cache, const b200l_kv_rows* rows, const int64_t* slots,
                               int64_t tokens, void* stream);
 
-/* The values of n slots, code * scale rounded once to dtype: k_out and v_out
+/* The values of n slots, code * scale in fp32, rounded to dtype: k_out and v_out
  * are [n, num_heads, head_dim], contiguous, 16-byte aligned where head_dim is a
  * multiple of 8. Slots outside the cache read as 0. */
 B200L_API int b200l_kv_read(const b200l_kv_cache* cache, const int64_t* slots, int64_t n, void* k_out, void* v_out,
@@ -380,7 +380,8 @@ B200L_API int b200l_kv_read(const b200l_kv_cache* cache, const int64_t* slots, i
  * reads key/value head h / (num_heads / cache heads). A row that sees no key is
  * 0, as are the rows from cu_new[requests] on. Keys behind block table entries
  * outside the cache are not there. A request with more than max_new new tokens
- * has not-a-number in the rows that the kernel chosen by max_new does not take. */
+ * has not-a-number in the rows that the kernel chosen by max_new does not take.
+ * Value scales below 2^-100 count as 2^-100. */
 typedef struct b200l_kv_attn_desc {
     const void* q;              /* [tokens, num_heads, head_dim], dims contiguous */
     void* out;                  /* the same shape, contiguous */
