@@ -25,11 +25,13 @@ def _beside_the_capture(device: torch.device) -> Iterator[torch.cuda.Stream]:
     mode = ctypes.c_int32(_lib.CAPTURE_RELAXED)
     _lib.check(_lib.lib().b200l_exchange_capture_mode(ctypes.byref(mode)))
     try:
-        capturing = True
-        while capturing:                        # (torch hands out the same few streams in turn)
+        for _ in range(64):                     # (torch hands out the same 32 streams in turn)
             stream = torch.cuda.Stream(device)
             with torch.cuda.stream(stream):
-                capturing = torch.cuda.is_current_stream_capturing()
+                if not torch.cuda.is_current_stream_capturing():
+                    break
+        else:
+            raise RuntimeError("every stream is being captured: run the step once before its capture")
         with torch.cuda.stream(stream):
             yield stream
     finally:

@@ -79,6 +79,17 @@ def test_an_outgrown_workspace_is_kept_if_a_capture_used_it(pkg, fake, stack):
     assert len(fake.cleared) == 5
 
 
+def test_no_stream_beside_the_captured_ones(pkg, fake, monkeypatch):
+    """An error and not an endless search, and the thread's capture mode is put back."""
+    layer = pkg.B200TransformerLayer(32, 1)
+    modes = []
+    fake.b200l_exchange_capture_mode = lambda mode: modes.append(mode) or 0
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        grow(layer, fake, 4096)
+    assert len(modes) == 2 and layer._ws is None
+
+
 def test_threads_take_turns_at_a_streams_workspace(pkg, monkeypatch):
     """A call's launches pass numbers through the workspace: no other thread's call on the
     same stream comes between them, nor between the choice of a buffer and its use; calls
